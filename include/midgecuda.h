@@ -143,6 +143,93 @@ int mg_moe_ffn_noalloc(const mg_expert_layout *L, const uint8_t *experts, int la
 int mg_sample_topp(const float *logits, int64_t ldl, int64_t V, int n_rows, float temp, float top_p, uint64_t *rng,
                    int32_t *out, float *probs, void *stream);
 
+/* ---- 4-bit paged key/value cache and token scoring (no counterpart in the
+ * reference, whose cache is f16 and contiguous, engine/midge.c:267-273, and
+ * which reports logits only).  Rows of activations (queries, keys, values,
+ * outputs, logits) are f32, f16 or bf16; sums, softmax statistics and norms
+ * are 32 bits or more whatever the type. */
+enum { MG_ACT_F32 = 0, MG_ACT_F16 = 1, MG_ACT_BF16 = 2 };
+
+/* A layer's cache: a pool of pages shared by n_seqs sequences.  Position p of
+ * sequence s lies in page table[s * ld_table + p / page_size] (device int32;
+ * entries beyond a sequence's length are not used, entries outside the pool
+ * are clamped to it).  A page holds keys and values of page_size positions of
+ * every key/value head as e2m1 codes with one e5m2 scale per position and 32
+ * dimensions: 4.25 bits a number, 34 head_dim bytes per 32 positions and
+ * head, in the order of tensor-core fragments (midge_b200/csrc/mg_kv4.cuh).
+ * Pages need no clearing.  head_dim 64 or 128, page_size a multiple of 32 up
+ * to 4096, pages 16-byte aligned. */
+typedef struct {
+    int n_kv_heads, head_dim, page_size, n_seqs;
+    int64_t n_pages;
+    void *pages;            /* device, n_pages * mg_kv4_page_bytes() bytes */
+    const int32_t *table;   /* device, [n_seqs x ld_table] */
+    int64_t ld_table;       /* entries of a sequence: at most ld_table * page_size positions */
+} mg_kv4;
+
+/* Bytes of one page, or a negative MG_ERR_*. */
+int64_t mg_kv4_page_bytes(int n_kv_heads, int head_dim, int page_size);
+
+/* Store n_tok tokens' keys and values (rows of n_kv_heads * head_dim) and
+ * write the queries (rows of n_heads * head_dim; n_heads may be 0) to q_out:
+ * queries and keys take a per-head RMSNorm where q_norm / k_norm (head_dim
+ * floats, or NULL) is given, x / sqrt(mean x^2 + eps) * w, then the half-split
+ * rotation by row tok_pos of rope_cos / rope_sin ([rope_rows x head_dim / 2]
+ * floats, or both NULL); values are stored as they are.  Token t belongs to
+ * sequence tok_seq[t] (NULL: 0) at position tok_pos[t]; no two tokens of a
+ * call share a place.  A token whose position is negative (padding), or whose
+ * sequence or position lies outside the table or the rotation, is skipped:
+ * nothing of it is stored or written.  q_out may be q.  A group's scale is
+ * the least e5m2 number >= its largest magnitude / 6, between 2^-14 and
+ * 10240; codes round to nearest, ties to even; magnitudes above 61440 (and
+ * infinities) saturate, NaN is stored as 0.  The first write of a position
+ * and every later one are alike, so a call may be repeated. */
+int mg_kv4_append(const mg_kv4 *c, int act, int n_tok, int n_heads, const void *q, int64_t ldq, const void *k,
+                  int64_t ldk, const void *v, int64_t ldv, const float *q_norm, const float *k_norm, float eps,
+                  const float *rope_cos, const float *rope_sin, int64_t rope_rows, const int32_t *tok_seq,
+                  const int32_t *tok_pos, void *q_out, int64_t ldqo, void *stream);
+
+/* The numbers the cache holds for n_tok stored positions (sequences tok_seq,
+ * NULL: 0), as rows of n_kv_heads * head_dim; k or v may be NULL.  Exact in
+ * every type.  A position outside the table gives zeros. */
+int mg_kv4_read(const mg_kv4 *c, int act, int n_tok, const int32_t *tok_seq, const int32_t *tok_pos, void *k,
+                int64_t ldk, void *v, int64_t ldv, void *stream);
+
+/* Attention of new queries over the cache.  Sequence s has the query rows
+ * q_start[s] .. q_start[s + 1] - 1 (device int32 [n_seqs + 1], not falling)
+ * and kv_len[s] cached positions (device int32), its queries' own included;
+ * its query j of n stands at position p = kv_len - n + j and sees the
+ * positions <= p, and with window > 0 only those > p - window.  Query head h
+ * reads key/value head h / (n_heads / n_kv_heads); n_heads is a multiple of
+ * n_kv_heads, up to 64 times it.  sinks (device, n_heads floats, or NULL) are
+ * logits that join each softmax without a value.  A query that sees nothing
+ * gets zeros.  max_q >= every number of queries (rows beyond it are not
+ * written) and max_kv, about the longest kv_len, choose the kernel and its
+ * split; any kv_len up to ld_table * page_size is right.
+ * work: mg_kv4_attn_work() bytes of device memory, zero before its first use;
+ * a call leaves it ready for the next on the same stream, of whatever
+ * sizes it is large enough for.  Calls that overlap in time need a workspace
+ * each. */
+int64_t mg_kv4_attn_work(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv);
+int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q, int64_t ldq, const int32_t *q_start,
+                const int32_t *kv_len, int max_q, int64_t max_kv, float scale, int window, const float *sinks,
+                void *out, int64_t ldo, void *work, int64_t work_bytes, void *stream);
+
+/* Per logits row (row i at logits + i * ldl, V entries): the natural-log
+ * probabilities of its n_ids given tokens ids[i * n_ids ..] (an id outside
+ * 0 .. V - 1 marks no token: 0), the entropy of its distribution, and its
+ * n_alt <= MG_LOGPROBS_MAX_ALT most probable tokens with their log
+ * probabilities, by value and then by index (with V < n_alt the rest is -1
+ * and -infinity).  A logit of -infinity has probability 0 and may be an
+ * alternative; NaN counts as -infinity.  A row of nothing but -infinity has
+ * log probabilities -infinity and entropy 0; one with +infinity has NaN.  lp [n_rows x n_ids], entropy
+ * [n_rows], alt_ids / alt_lp [n_rows x n_alt].  work as for mg_kv4_attn. */
+#define MG_LOGPROBS_MAX_ALT 32
+int64_t mg_logprobs_work(int64_t V, int n_rows, int n_alt);
+int mg_logprobs(int act, const void *logits, int64_t ldl, int64_t V, int n_rows, const int32_t *ids, int n_ids,
+                int n_alt, float *lp, float *entropy, int32_t *alt_ids, float *alt_lp, void *work,
+                int64_t work_bytes, void *stream);
+
 /* Failure-path self-test of a bounded device wait (no counterpart in the
  * reference): a one-CTA kernel waits `polls` times (1..2^20) on an mbarrier
  * that nothing arrives on, records the timeout in the library's error word,

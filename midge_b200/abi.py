@@ -17,6 +17,7 @@ LIB_PATH = os.path.join(PKG, "libmidgecuda.so")
 
 MG_F32, MG_Q8R, MG_Q4G32, MG_MXFP4 = 0, 1, 2, 3
 MG_SCALE_F16, MG_SCALE_UE8M0 = 0, 1
+MG_ACT_F32, MG_ACT_F16, MG_ACT_BF16 = 0, 1, 2
 MG_OK, MG_ERR_ARG, MG_ERR_CUDA, MG_ERR_OOM, MG_ERR_STATE, MG_ERR_RANGE, MG_ERR_SPEC = 0, -1, -2, -3, -4, -5, -6
 MG_ERR_TIMEOUT, MG_ERR_COMM = -8, -9
 EP_ID_BYTES = 128
@@ -44,6 +45,12 @@ class MgSpec(C.Structure):
 class MgExpertLayout(C.Structure):
     _fields_ = [("dt", i32), ("scale_fmt", i32), ("hidden", i64), ("ffn", i64),
                 ("off", (i64 * 3) * 3), ("expert_stride", i64), ("layer_stride", i64)]
+
+
+class MgKv4(C.Structure):
+    """A layer's 4-bit paged key/value cache (device pointers)."""
+    _fields_ = [("n_kv_heads", i32), ("head_dim", i32), ("page_size", i32), ("n_seqs", i32), ("n_pages", i64),
+                ("pages", vp), ("table", vp), ("ld_table", i64)]
 
 
 class MidgeError(RuntimeError):
@@ -98,6 +105,15 @@ def _load():
         "mg_sample_topp": (i32, [vp, i64, i64, i32, f32, f32, vp, vp, vp, vp]),
         "mg_model_sample": (i32, [vp, i32, f32, f32, vp, vp]),
         "mg_model_put_logits": (i32, [vp, i32, vp]),
+        "mg_kv4_page_bytes": (i64, [i32, i32, i32]),
+        "mg_kv4_append": (i32, [C.POINTER(MgKv4), i32, i32, i32, vp, i64, vp, i64, vp, i64, vp, vp, f32, vp, vp, i64,
+                                vp, vp, vp, i64, vp]),
+        "mg_kv4_read": (i32, [C.POINTER(MgKv4), i32, i32, vp, vp, vp, i64, vp, i64, vp]),
+        "mg_kv4_attn_work": (i64, [C.POINTER(MgKv4), i32, i32, i64]),
+        "mg_kv4_attn": (i32, [C.POINTER(MgKv4), i32, i32, vp, i64, vp, vp, i32, i64, f32, i32, vp, vp, i64, vp, i64,
+                              vp]),
+        "mg_logprobs_work": (i64, [i64, i32, i32]),
+        "mg_logprobs": (i32, [i32, vp, i64, i64, i32, vp, i32, i32, vp, vp, vp, vp, vp, i64, vp]),
         "mg_wait_selftest": (i32, [i32, C.POINTER(i32)]),
         "mg_model_ep_stats": (i32, [vp, vp]),
     }
@@ -118,6 +134,13 @@ def check(rc):
     if rc != MG_OK:
         raise MidgeError(rc, (lib.mg_last_error() or b"").decode())
     return rc
+
+
+def check_size(n):
+    """The byte count a sizing entry point returned, or its error raised."""
+    if n < 0:
+        check(int(n))
+    return int(n)
 
 
 def make_spec(spec: dict):

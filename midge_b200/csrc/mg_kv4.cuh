@@ -1,0 +1,121 @@
+// mg_kv4.cuh -- the 4-bit paged key/value cache: its layout, its codes and
+// the activation types of the operators on it.
+//
+// A page holds, for each key/value head, page_size / 32 tiles of 32
+// positions; a tile of head_dim D (64 or 128) has G = D / 32 groups of 32
+// dimensions per position and 32 D + 64 G = 34 D bytes:
+//   [0, 16 D)      keys: e2m1 codes, two per byte, the even dimension low
+//   [16 D, 32 D)   values, the same
+//   [32 D, 33 D)   the keys' scales: an e5m2 byte per position and group
+//   [33 D, 34 D)   the values' scales
+// A stored number is code x scale: at most 2 + 3 significant bits, so it is
+// exact in f16 (the e5m2 byte is the high byte of the scale's f16).
+//
+// The codes lie in the order in which a lane of an mma.m16n8k16 warp reads
+// them, lane = 4 g + t.  Keys (B operand, n = position, k = dimension): the
+// lane holds positions 16 u + 2 g + j and the dimensions [t D/4, (t+1) D/4).
+// Values (B operand, n = dimension, k = position): the lane holds positions
+// 16 u + 4 t + i, i = c + 2 s, and the dimensions [g D/8, (g+1) D/8).  A lane
+// reads both in 16-byte pieces, 512 bytes per warp and piece:
+//   keys   D = 64:  piece u,       16 bytes = j (2) x 8
+//          D = 128: piece 2 u + j, 16 bytes
+//   values D = 64:  piece u,       16 bytes = i (4) x 4
+//          D = 128: piece 2 u + c, 16 bytes = s (2) x 8
+// and scales in words: keys [g][group][u][j], values [t][group][u][i].
+#pragma once
+#include <cuda_bf16.h>
+
+#include "mg_common.cuh"
+
+namespace mg {
+
+constexpr int KV4_TILE = 32;  // positions of a tile
+
+__host__ __device__ constexpr int kv4_tile_bytes(int hd) { return 34 * hd; }
+
+// byte of position p's (0..31) dimension d within the tile; nibble d & 1
+template <int HD>
+__device__ __forceinline__ int kv4_k_code(int p, int d) {
+    const int u = p >> 4, g = (p >> 1) & 7, j = p & 1;
+    if (HD == 64) return u * 512 + (g * 4 + (d >> 4)) * 16 + j * 8 + ((d & 15) >> 1);
+    return (2 * u + j) * 512 + (g * 4 + (d >> 5)) * 16 + ((d & 31) >> 1);
+}
+template <int HD>
+__device__ __forceinline__ int kv4_v_code(int p, int d) {
+    const int u = p >> 4, t = (p >> 2) & 3, i = p & 3;
+    if (HD == 64) return 16 * HD + u * 512 + ((d >> 3) * 4 + t) * 16 + i * 4 + ((d & 7) >> 1);
+    return 16 * HD + (2 * u + (i & 1)) * 512 + ((d >> 4) * 4 + t) * 16 + (i >> 1) * 8 + ((d & 15) >> 1);
+}
+template <int HD>
+__device__ __forceinline__ int kv4_k_scale(int p, int grp) {
+    return 32 * HD + (((p >> 1) & 7) * (HD / 32) + grp) * 4 + ((p >> 4) << 1) + (p & 1);
+}
+template <int HD>
+__device__ __forceinline__ int kv4_v_scale(int p, int grp) {
+    return 33 * HD + ((((p >> 2) & 3) * (HD / 32) + grp) * 2 + (p >> 4)) * 4 + (p & 3);
+}
+
+__device__ __forceinline__ float e5m2_f32(uint32_t byte) { return h2f((uint16_t)(byte << 8)); }
+__device__ __forceinline__ float e2m1_f32(uint32_t nib) {
+    const uint32_t h = e2m1x2_to_h2(nib & 15u);
+    return h2f((uint16_t)h);
+}
+
+// The scale of a group of largest magnitude `top`: the least e5m2 value s
+// with 6 s >= top, from 2^-14 (the least normal; anything below half its
+// least code rounds to zero, as the f16 cache flushes subnormals) to 10240
+// (larger numbers saturate at 61440, where f16 would overflow); 0 for top = 0.
+__device__ __forceinline__ uint32_t kv4_scale(float top) {
+    if (!(top > 0.f)) return 0u;
+    // an estimate of the byte from top / 6, then one step either way by exact products (6 s has 4 significant bits)
+    const float est = fminf(fmaxf(top * (1.0f / 6.0f), 6.103515625e-5f), 10240.f);
+    uint32_t b = (__float_as_uint(est) >> 21) - (112u << 2);
+    if (b < 0x71u && e5m2_f32(b) * 6.f < top) b++;
+    if (b > 4u && e5m2_f32(b - 1) * 6.f >= top) b--;
+    return b;
+}
+// The nearest e2m1 code of x / s, ties to the even code: |x| against the
+// exact products s x midpoint (s has 3 significant bits, the midpoints 3).
+// s = 0 gives code 0.
+__device__ __forceinline__ uint32_t kv4_code(float x, float s) {
+    const float a = fabsf(x);
+    uint32_t c = (a > 0.25f * s) + (a >= 0.75f * s) + (a > 1.25f * s) + (a >= 1.75f * s) + (a > 2.5f * s) +
+                 (a >= 3.5f * s) + (a > 5.f * s);
+    if (!(s > 0.f)) c = 0;
+    return c | (x < 0.f ? 8u : 0u);
+}
+
+// ------------------------------------------------------- activation types
+template <int ACT> struct Act;
+template <> struct Act<MG_ACT_F32> { using T = float; };
+template <> struct Act<MG_ACT_F16> { using T = __half; };
+template <> struct Act<MG_ACT_BF16> { using T = __nv_bfloat16; };
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <typename T> __device__ __forceinline__ T from_f32(float x);
+template <> __device__ __forceinline__ float from_f32<float>(float x) { return x; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+
+// The cache as the kernels take it.  Table entries are clamped to the pool,
+// so that a stale entry reads another page but never outside the pool.
+struct Kv4 {
+    uint8_t *pages;
+    const int32_t *table;
+    int64_t ld_table, head_bytes;  // head_bytes: one key/value head of one page
+    int n_kv, page, n_seqs;
+    int n_pages;
+    int64_t cap;                   // positions the table's rows cover
+    // tile of positions [32 tile, 32 tile + 32) of sequence seq, key/value head h
+    __device__ __forceinline__ uint8_t *tile(int seq, int h, int tile, int tile_bytes) const {
+        const int per = page >> 5, pg = tile / per;
+        int id = table[(int64_t)seq * ld_table + pg];
+        id = id < 0 ? 0 : (id >= n_pages ? n_pages - 1 : id);
+        return pages + ((int64_t)id * n_kv + h) * head_bytes + (int64_t)(tile - pg * per) * tile_bytes;
+    }
+};
+int kv4_take(const mg_kv4 *c, Kv4 *out);  // checks the geometry (mg_kv4.cu)
+
+}  // namespace mg
