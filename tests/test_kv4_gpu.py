@@ -378,7 +378,7 @@ def test_append_then_attend_in_a_graph(torch_cuda):
     pos, kl = torch.tensor([59, 30], dtype=torch.int32, device="cuda"), torch.tensor([60, 31], dtype=torch.int32, device="cuda")
     seq = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
     qs = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
-    work = torch.zeros(1 << 22, dtype=torch.uint8, device="cuda")
+    work = torch.zeros(abi.check_size(abi.lib.mg_kv4_attn_work(dev.ref(), 8, 1, 96)), dtype=torch.uint8, device="cuda")
     co, si = (torch.from_numpy(x).cuda() for x in rope(96, 64))
     P = lambda t: t.data_ptr()  # noqa: E731
 
