@@ -15,41 +15,48 @@ namespace mg {
 
 // ------------------------------------------------------------------ few rows
 // A row is a (query, head) pair of one key/value head: row r = j gq + h.  The
-// kernel holds 8 rows (f32) or 8 or 16 rows (f16, bf16) as the A operand of
-// mma.m16n8k16 and streams tiles of 32 positions:
+// kernel holds 8 rows (16 for f16 and bf16 where there are more than 8) and
+// streams tiles of 32 positions:
 //   * one bulk copy per tile into a ring of the warp's own (a tile with its
-//     scales is contiguous in the cache), NST ahead;
+//     scales is contiguous in the cache), KD_NST - 1 ahead;
 //   * codes -> f16 in registers (cvt.f16x2.e2m1x2, then the scale: exact),
-//     straight in the order of the B fragments;
-//   * scores, a running maximum and sum per row (fp32, base 2), weights as A
-//     fragments from the score accumulators, no shared memory in between.
-// f32 queries and weights go as f16 hi and lo halves stacked in rows g and
-// g + 8 of the same MMA (22 bits; the sums of a tile start from zero and are
-// added in fp32, since the tensor core truncates its running sum).  f16 and
-// bf16 queries are exact in f16 after scaling by a power of two per row;
-// their weights are rounded to f16 (2^-11 of a weight: a quarter of the bf16
+//     straight in the order of mma.m16n8k16 fragments;
+//   * both products are transposed, S^T = K Q^T and O^T = V^T P^T: the 16-row
+//     operand is positions, then dimensions, and the rows are its 8 columns,
+//     so no part of an MMA is empty at 8 rows (half the MMAs of Q K^T: mma.sync
+//     runs at a quarter of the tcgen05 rate here, 8 cycles a scheduler);
+//   * weights go from score accumulators to B fragments by movmatrix.
+// f32 queries and weights go as f16 hi and lo halves in two MMAs into the
+// same accumulator (22 bits; a tile's sums start from zero and are added in
+// fp32, since the tensor core truncates its running sum).  f16 and bf16
+// queries are exact in f16 after scaling by a power of two per row; their
+// weights are rounded to f16 (2^-11 of a weight: a quarter of the bf16
 // result's own rounding).
 //
-// Work: all tiles of all (sequence, key/value head, row group) in one line,
-// cut evenly over the blocks, whatever the lengths; a block's warps take
-// every tile of a segment in turn.  A (sequence, head) that lies in
-// several blocks is joined by the last of them to finish, in block order, so
-// results do not depend on the order of arrival.
+// Work: a unit is a (sequence, key/value head, row group); units of more than
+// `chunk` tiles are cut into equal pieces, chunk coming from the tiles of the
+// whole call, so that the pieces are alike whatever the lengths.  A block
+// takes a piece, its warps the piece's tiles in turn.  A cut unit is joined by
+// the last of its blocks to finish, in piece order, so results do not depend
+// on the order of arrival.
 constexpr int KD_NST = 4;    // ring stages of a warp
-constexpr int KD_CTAS = 2;   // blocks of an SM
 constexpr int KD_ERR = 41;
-__host__ __device__ constexpr int kd_warps(int hd) { return hd == 64 ? 8 : 6; }  // 128 and 168 registers a thread
+constexpr int KD_WARPS_LONG = 4, KD_WARPS_SHORT = 2;  // warps of a block
+constexpr int KD_MIN_CHUNK = 16;                      // tiles worth a piece of their own
+constexpr int KD_MAX_CUT = 128;                       // pieces of a unit
+__host__ __device__ constexpr int kd_warps_sm(int hd) { return hd == 64 ? 16 : 12; }  // 128 and 168 registers a thread
 
 enum { KD_SPLIT = 0, KD_ROWS8 = 1, KD_ROWS16 = 2 };
 __host__ __device__ constexpr int kd_rows(int mode) { return mode == KD_ROWS16 ? 16 : 8; }
-template <int HD> constexpr size_t kd_smem() { return (size_t)kd_warps(HD) * KD_NST * kv4_tile_bytes(HD); }
+template <int HD> constexpr size_t kd_smem(int warps) { return (size_t)warps * KD_NST * kv4_tile_bytes(HD); }
 
+constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// the scale byte b of a word as f16x2 (both halves); two bytes of a word as a pair
+// the scale byte b of a word as f16x2, both halves
 __device__ __forceinline__ uint32_t scale_h2(uint32_t w, int b) { return __byte_perm(w, 0u, (b << 12) | (b << 4) | 0x404); }
 __device__ __forceinline__ uint32_t h2_rn(float lo, float hi) {
     const __half2 h = __floats2half2_rn(lo, hi);
@@ -62,6 +69,21 @@ __device__ __forceinline__ void split_h2(float a, float b, uint32_t &hi, uint32_
     hi = *reinterpret_cast<const uint32_t *>(&h);
     lo = h2_rn(a - f.x, b - f.y);
 }
+// the transpose of an 8 x 8 f16 matrix held as lane (row lane / 4, columns 2 (lane % 4), + 1)
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
+    return r;
+}
+__device__ __forceinline__ void mma4(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    const uint32_t a[4] = {a0, a1, a2, a3};
+    mma_16816(d, a, b0, b1);
+}
+
+// a / b; both below 2^32 but for caches of terabytes
+__device__ __forceinline__ long long div_line(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+}
 
 // keep of the four scale bytes of positions p .. p + 3 those in [first, len)
 __device__ __forceinline__ uint32_t live_bytes(uint32_t w, int p, int first, int len) {
@@ -71,91 +93,128 @@ __device__ __forceinline__ uint32_t live_bytes(uint32_t w, int p, int first, int
     return w;
 }
 
-template <int HD, int MODE, typename T>
-__global__ void __launch_bounds__(kd_warps(HD) * 32, KD_CTAS) k_kv4_attn_few(Kv4AttnArgs a) {
-    constexpr int KD_WARPS = kd_warps(HD), KD_THREADS = KD_WARPS * 32;
-    constexpr int ROWS = kd_rows(MODE), TB = kv4_tile_bytes(HD), KS = HD / 16, NT = HD / 8, G = HD / 32;
-    constexpr int RS = MODE == KD_ROWS16 ? 2 : 1;    // row sets of a lane: g, g + 8
-    constexpr int OC = MODE == KD_ROWS16 ? 4 : 2;    // output values of a lane per n-tile
+// N consecutive elements as floats; 16 bytes at a time where the row allows
+template <int N, typename T>
+__device__ __forceinline__ void load_row(const T *src, bool wide, float x[N]) {
+    if (wide) {
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N / V; i++) {
+            const uint4 v = reinterpret_cast<const uint4 *>(src)[i];
+            T e[V];
+            memcpy(e, &v, 16);
+#pragma unroll
+            for (int k = 0; k < V; k++) x[V * i + k] = to_f32(e[k]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = to_f32(src[i]);
+    }
+}
+template <typename T> __device__ __forceinline__ void store4f(T *dst, bool wide, float4 v) {
+    T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+    if (wide) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<uint4 *>(e);
+        else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<uint2 *>(e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) dst[i] = e[i];
+    }
+}
+
+template <int HD, int MODE, typename T, int KD_WARPS>
+__global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_kv4_attn_few(Kv4AttnArgs a) {
+    constexpr int KD_THREADS = KD_WARPS * 32;
+    constexpr int ROWS = kd_rows(MODE), SETS = ROWS / 8, TB = kv4_tile_bytes(HD), KS = HD / 16, G = HD / 32;
+    constexpr int MT = HD / 16;                    // O^T tiles of 16 dimensions
+    constexpr int QR = MODE == KD_SPLIT ? 4 : 2;   // query registers of a k-step: b0, b1 (and their lo halves)
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ uint64_t bars[KD_WARPS][KD_NST];
-    __shared__ long long s_scan[KD_WARPS + 1];
-    __shared__ long long s_off;
-    __shared__ int s_seq, s_last;
+    __shared__ long long s_sum[KD_WARPS];
+    __shared__ int2 s_scan[KD_WARPS];
+    __shared__ Kv4Seq s_q;
+    __shared__ int s_seq, s_off, s_slot, s_last;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     uint8_t *ring = smem + (size_t)warp * KD_NST * TB;
-    // a warp's result of a segment, in its own ring once that is drained: per row m, l, o[HD]
-    float *comb = reinterpret_cast<float *>(ring);
-    constexpr int COMB = KD_NST * TB / 4;  // floats from one warp's to the next
-    static_assert(ROWS * (HD + 2) <= COMB, "a warp's result fits its ring");
     if (lane == 0) {
         for (int i = 0; i < KD_NST; i++) mbar_init(&bars[warp][i], 1);
         fence_mbar_init();
     }
-    if (tid == 0) s_seq = -1;
 
-    // ---- this block's share of the line of tiles
-    const int n = a.c.n_seqs, per = (n + KD_THREADS - 1) / KD_THREADS;
-    long long mine = 0;
-    for (int s = tid * per; s < min(n, (tid + 1) * per); s++) {
-        Kv4Seq q;
+    // ---- the pieces: tiles of all sequences, then pieces before each sequence
+    const int n = a.c.n_seqs, per = (n + KD_THREADS - 1) / KD_THREADS, s0 = tid * per, s1 = min(n, s0 + per);
+    Kv4Seq q;
+    long long sum = 0;
+    for (int s = s0; s < s1; s++) {
         q.load(a, s);
-        mine += (long long)q.tiles * q.groups(a.gq, ROWS) * a.c.n_kv;
+        sum += (long long)q.tiles * q.groups(a.gq, ROWS) * a.c.n_kv;
     }
-    long long incl = mine;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (lane == 0) s_sum[warp] = sum;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int w = 0; w < KD_WARPS; w++) sum += s_sum[w];
+    const int chunk = (int)max((long long)KD_MIN_CHUNK, div_line(sum + a.pieces - 1, a.pieces));
+    auto cuts = [&](const Kv4Seq &q) { return min(KD_MAX_CUT, (q.tiles + chunk - 1) / chunk); };
+    int2 mine = make_int2(0, 0);  // pieces; pieces of cut units
+    for (int s = s0; s < s1; s++) {
+        if (per > 1) q.load(a, s);
+        const int c = cuts(q), all = c * q.groups(a.gq, ROWS) * a.c.n_kv;
+        mine.x += all;
+        mine.y += c > 1 ? all : 0;
+    }
+    int2 excl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long v = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += v;
+        const int x = __shfl_up_sync(0xffffffffu, excl.x, o), y = __shfl_up_sync(0xffffffffu, excl.y, o);
+        if (lane >= o) {
+            excl.x += x;
+            excl.y += y;
+        }
     }
-    if (lane == 31) s_scan[warp] = incl;
+    if (lane == 31) s_scan[warp] = excl;
     __syncthreads();
-    long long before = 0, total = 0;
+    excl.x -= mine.x;
+    excl.y -= mine.y;
+    int total = 0;
 #pragma unroll
     for (int w = 0; w < KD_WARPS; w++) {
-        before += w < warp ? s_scan[w] : 0;
-        total += s_scan[w];
-    }
-    // block b has the tiles [total b / nb, total (b + 1) / nb); tile y is block ((y + 1) nb - 1) / total's
-    const long long nb = min((long long)gridDim.x, total), b = blockIdx.x;
-    const long long begin = b < nb ? total * b / nb : 0, end = b < nb ? total * (b + 1) / nb : 0;
-    if (begin < end) {
-        const long long excl = before + incl - mine;
-        if (begin >= excl && begin < excl + mine) {
-            long long at = excl;
-            for (int s = tid * per;; s++) {
-                Kv4Seq q;
-                q.load(a, s);
-                const long long c = (long long)q.tiles * q.groups(a.gq, ROWS) * a.c.n_kv;
-                if (begin < at + c) {
-                    s_seq = s;
-                    s_off = begin - at;
-                    break;
-                }
-                at += c;
-            }
+        if (w < warp) {
+            excl.x += s_scan[w].x;
+            excl.y += s_scan[w].y;
         }
+        total += s_scan[w].x;
     }
-    __syncthreads();
-    if (begin >= end) return;  // the whole block; nothing is in flight
 
-    int seq = s_seq;
-    long long off = s_off, cur = begin;
     uint32_t phase = 0;  // bit i: parity of ring stage i's next completion
     bool ok = true;
-    while (cur < end) {
-        Kv4Seq q;
-        q.load(a, seq);
-        const int groups = q.groups(a.gq, ROWS);
-        const long long cnt = (long long)q.tiles * groups * a.c.n_kv;
-        if (off >= cnt) {
-            off -= cnt;
-            seq++;
-            continue;
+    for (int piece = blockIdx.x; piece < total; piece += gridDim.x) {
+        if (piece >= excl.x && piece < excl.x + mine.x) {
+            int at = excl.x, slot = excl.y;
+            for (int s = s0;; s++) {
+                Kv4Seq qq;
+                qq.load(a, s);
+                const int c = cuts(qq), all = c * qq.groups(a.gq, ROWS) * a.c.n_kv;
+                if (piece < at + all) {
+                    s_q = qq;
+                    s_seq = s;
+                    s_off = piece - at;
+                    s_slot = slot;
+                    break;
+                }
+                at += all;
+                slot += c > 1 ? all : 0;
+            }
         }
-        const int hr = (int)(off / q.tiles), ta = (int)(off - (long long)hr * q.tiles);
+        __syncthreads();
+        const int seq = s_seq;
+        const Kv4Seq q = s_q;
+        const int groups = q.groups(a.gq, ROWS), ncut = cuts(q);
+        const int hr = s_off / ncut, cut = s_off - hr * ncut;
         const int kh = hr / groups, rg = hr - kh * groups;
-        const int nt = (int)min((long long)(q.tiles - ta), end - cur);  // tiles of this segment
+        const int ta = (int)((long long)q.tiles * cut / ncut), nt = (int)((long long)q.tiles * (cut + 1) / ncut) - ta;
         const int tile_a = q.tile0 + ta;
         const int wt = nt > warp ? (nt - warp + KD_WARPS - 1) / KD_WARPS : 0;  // this warp's tiles of it
 
@@ -176,57 +235,70 @@ __global__ void __launch_bounds__(kd_warps(HD) * 32, KD_CTAS) k_kv4_attn_few(Kv4
                 bulk_g2s(ring + (size_t)(i % KD_NST) * TB, reinterpret_cast<const void *>(p), TB, &bars[warp][i % KD_NST]);
             }
         };
-        // a segment starts at stage 0 again; `phase` carries the parities
         look_up(0);
+
+        // ---- the queries as B fragments (lane: row g, dimensions t HD / 4 ..); loaded before the copies wait for the table
+        uint32_t qb[SETS][KS][QR];
+        float own_factor[SETS];
+        float x[SETS][HD / 4];
+#pragma unroll
+        for (int s = 0; s < SETS; s++) {
+            const int r = rg * ROWS + 8 * s + g, j = r / a.gq, h = kh * a.gq + r - j * a.gq;
+            if (j < q.nq) {
+                load_row<HD / 4>(static_cast<const T *>(a.q) + (int64_t)(q.q0 + j) * a.ldq + (int64_t)h * HD + t * (HD / 4),
+                                 a.q_wide, x[s]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < HD / 4; i++) x[s][i] = 0.f;
+            }
+        }
+        // every piece starts at stage 0; `phase` carries the parities
 #pragma unroll
         for (int i = 0; i < KD_NST - 1; i++) issue(i);
-
-        // ---- the rows: queries as A fragments, per-row limits and factors
-        uint32_t qa[KS][MODE == KD_ROWS8 ? 2 : 4];
-        float m[RS], l[RS], factor[RS];
-        int hi[RS], lo[RS];
 #pragma unroll
-        for (int s = 0; s < RS; s++) {
-            const int r = rg * ROWS + g + 8 * s, j = r / a.gq, h = kh * a.gq + r - j * a.gq;
-            const bool live = j < q.nq;
-            hi[s] = live ? q.len - q.nq + j : -1;
-            lo[s] = a.window > 0 ? hi[s] - a.window + 1 : 0;
-            m[s] = -INFINITY;
-            l[s] = 0.f;
-            const T *src = static_cast<const T *>(a.q) + (int64_t)(q.q0 + (live ? j : 0)) * a.ldq +
-                           (int64_t)(live ? h : 0) * HD + t * (HD / 4);
-            float x[HD / 4], top = 0.f;
+        for (int s = 0; s < SETS; s++) {
+            float top = 0.f;
 #pragma unroll
-            for (int i = 0; i < HD / 4; i++) {
-                x[i] = live ? to_f32(src[i]) : 0.f;
-                top = fmaxf(top, fabsf(x[i]));
-            }
+            for (int i = 0; i < HD / 4; i++) top = fmaxf(top, fabsf(x[s][i]));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // 2^-e, e = the exponent of the row's largest: the row's values are below 2 in f16
             const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
             const float down = __uint_as_float((254u - e) << 23);
-            factor[s] = a.scale * 1.4426950408889634f * __uint_as_float(e << 23);
+            own_factor[s] = a.scale * LOG2E * __uint_as_float(e << 23);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                const float x0 = x[4 * k] * down, x1 = x[4 * k + 1] * down, x2 = x[4 * k + 2] * down, x3 = x[4 * k + 3] * down;
+                const float x0 = x[s][4 * k] * down, x1 = x[s][4 * k + 1] * down;
+                const float x2 = x[s][4 * k + 2] * down, x3 = x[s][4 * k + 3] * down;
                 if constexpr (MODE == KD_SPLIT) {
-                    split_h2(x0, x1, qa[k][0], qa[k][1]);
-                    split_h2(x2, x3, qa[k][2], qa[k][3]);
-                } else if constexpr (MODE == KD_ROWS8) {
-                    qa[k][0] = h2_rn(x0, x1);
-                    qa[k][1] = h2_rn(x2, x3);
+                    split_h2(x0, x1, qb[s][k][0], qb[s][k][2]);
+                    split_h2(x2, x3, qb[s][k][1], qb[s][k][3]);
                 } else {
-                    qa[k][s] = h2_rn(x0, x1);
-                    qa[k][2 + s] = h2_rn(x2, x3);
+                    qb[s][k][0] = h2_rn(x0, x1);
+                    qb[s][k][1] = h2_rn(x2, x3);
                 }
             }
         }
-        float o[NT][OC];
+        // ---- the rows whose scores this lane holds: 8 s + 2 t + c
+        float m[SETS][2], l[SETS][2], factor[SETS][2];
+        int hi[SETS][2];
 #pragma unroll
-        for (int i = 0; i < NT; i++)
+        for (int s = 0; s < SETS; s++)
 #pragma unroll
-            for (int c = 0; c < OC; c++) o[i][c] = 0.f;
+            for (int c = 0; c < 2; c++) {
+                factor[s][c] = __shfl_sync(0xffffffffu, own_factor[s], (2 * t + c) * 4);
+                const int j = (rg * ROWS + 8 * s + 2 * t + c) / a.gq;
+                hi[s][c] = j < q.nq ? q.len - q.nq + j : -1;
+                m[s][c] = -INFINITY;
+                l[s][c] = 0.f;
+            }
+        float o[SETS][MT][4];  // dimension 2 MT g + 2 mt (+ 1: elements 2, 3), rows 2 t, 2 t + 1
+#pragma unroll
+        for (int s = 0; s < SETS; s++)
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) o[s][i][c] = 0.f;
 
 #pragma unroll 1
         for (int i = 0; i < wt; i++) {
@@ -237,8 +309,8 @@ __global__ void __launch_bounds__(kd_warps(HD) * 32, KD_CTAS) k_kv4_attn_few(Kv4
             const uint8_t *tb = ring + (size_t)st * TB;
             const int p0 = (tile_a + warp + i * KD_WARPS) * 32;
             const uint32_t ksc = *reinterpret_cast<const uint32_t *>(tb + 32 * HD + (g * G + t * G / 4) * 4);
-            // ---- scores of 32 positions: sc[u][j] holds columns 2t, 2t + 1 = positions 16 u + 4 t + j, + 2
-            float sc[2][2][4];
+            // ---- scores: sc[s][u][2 j + c] = position 16 u + 2 g + j, row 8 s + 2 t + c
+            float sc[SETS][2][4];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 uint32_t kw[2][HD / 32];
@@ -252,89 +324,96 @@ __global__ void __launch_bounds__(kd_warps(HD) * 32, KD_CTAS) k_kv4_attn_few(Kv4
                         kw[j][0] = v.x; kw[j][1] = v.y; kw[j][2] = v.z; kw[j][3] = v.w;
                     }
                 }
+                const uint32_t f0 = scale_h2(ksc, 2 * u), f1 = scale_h2(ksc, 2 * u + 1);
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const uint32_t f = scale_h2(ksc, 2 * u + j);
-                    float *d = sc[u][j];
-                    d[0] = d[1] = d[2] = d[3] = 0.f;
+                for (int s = 0; s < SETS; s++) sc[s][u][0] = sc[s][u][1] = sc[s][u][2] = sc[s][u][3] = 0.f;
 #pragma unroll
-                    for (int w = 0; w < HD / 32; w++) {
-                        uint32_t h[4];
-                        e2m1x8_to_h2(kw[j][w], h);
+                for (int w = 0; w < HD / 32; w++) {
+                    uint32_t h0[4], h1[4];
+                    e2m1x8_to_h2(kw[0][w], h0);
+                    e2m1x8_to_h2(kw[1][w], h1);
 #pragma unroll
-                        for (int k = 0; k < 2; k++) {
-                            uint32_t af[4];
-                            if constexpr (MODE == KD_ROWS8) {
-                                af[0] = qa[2 * w + k][0]; af[2] = qa[2 * w + k][1]; af[1] = af[3] = 0u;
-                            } else {
-#pragma unroll
-                                for (int c = 0; c < 4; c++) af[c] = qa[2 * w + k][c];
-                            }
-                            mma_16816(d, af, hmul2_u32(h[2 * k], f), hmul2_u32(h[2 * k + 1], f));
-                        }
+                    for (int k = 0; k < 4; k++) {
+                        h0[k] = hmul2_u32(h0[k], f0);
+                        h1[k] = hmul2_u32(h1[k], f1);
                     }
+#pragma unroll
+                    for (int k = 0; k < 2; k++)
+#pragma unroll
+                        for (int s = 0; s < SETS; s++) {
+                            const uint32_t *b = qb[s][2 * w + k];
+                            mma4(sc[s][u], h0[2 * k], h1[2 * k], h0[2 * k + 1], h1[2 * k + 1], b[0], b[1]);
+                            if constexpr (MODE == KD_SPLIT)
+                                mma4(sc[s][u], h0[2 * k], h1[2 * k], h0[2 * k + 1], h1[2 * k + 1], b[2], b[3]);
+                        }
                 }
             }
             // ---- weights
             // some row does not see some position: the last tiles, and with a window the first ones
             const bool edge = p0 + 32 > q.len - q.nq + 1 || (a.window > 0 && p0 < q.len - a.window);
-            uint32_t pa[2][4];
-            float alpha[RS];
+            uint32_t pb[SETS][2][QR];
+            float alpha[SETS][2];
 #pragma unroll
-            for (int s = 0; s < RS; s++) {
-                float x[2][2][2];
-                float top = -INFINITY;
+            for (int s = 0; s < SETS; s++) {
+                float mm[2];
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                for (int c = 0; c < 2; c++) {
+                    float top = -INFINITY;
 #pragma unroll
-                    for (int j = 0; j < 2; j++)
+                    for (int u = 0; u < 2; u++)
 #pragma unroll
-                        for (int c = 0; c < 2; c++) {
-                            float v = (MODE == KD_SPLIT ? sc[u][j][c] + sc[u][j][2 + c] : sc[u][j][2 * s + c]) * factor[s];
+                        for (int j = 0; j < 2; j++) {
+                            float &v = sc[s][u][2 * j + c];
+                            v *= factor[s][c];
                             if (edge) {
-                                const int p = p0 + 16 * u + 4 * t + j + 2 * c;
-                                v = p <= hi[s] && p >= lo[s] ? v : -INFINITY;
+                                const int p = p0 + 16 * u + 2 * g + j;
+                                v = p <= hi[s][c] && (a.window == 0 || p > hi[s][c] - a.window) ? v : -INFINITY;
                             }
-                            x[u][j][c] = v;
                             top = fmaxf(top, v);
                         }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float mn = fmaxf(m[s], top), mm = mn == -INFINITY ? 0.f : mn;
-                alpha[s] = ex2(m[s] - mm);
-                m[s] = mn;
-                float sum = 0.f;
+#pragma unroll
+                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+                    const float mn = fmaxf(m[s][c], top);
+                    mm[c] = mn == -INFINITY ? 0.f : mn;
+                    alpha[s][c] = ex2(m[s][c] - mm[c]);
+                    m[s][c] = mn;
+                    l[s][c] *= alpha[s][c];
+                }
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        const float e0 = ex2(x[u][j][0] - mm), e1 = ex2(x[u][j][1] - mm);
-                        sum += e0 + e1;
-                        if constexpr (MODE == KD_SPLIT) split_h2(e0, e1, pa[u][2 * j], pa[u][2 * j + 1]);
-                        else pa[u][2 * j + s] = h2_rn(e0, e1);
+                        const float e0 = ex2(sc[s][u][2 * j] - mm[0]), e1 = ex2(sc[s][u][2 * j + 1] - mm[1]);
+                        l[s][0] += e0;
+                        l[s][1] += e1;
+                        if constexpr (MODE == KD_SPLIT) {
+                            uint32_t h, r;
+                            split_h2(e0, e1, h, r);
+                            pb[s][u][j] = transpose8(h);
+                            pb[s][u][2 + j] = transpose8(r);
+                        } else {
+                            pb[s][u][j] = transpose8(h2_rn(e0, e1));
+                        }
                     }
-                if constexpr (MODE == KD_ROWS8) pa[0][1] = pa[0][3] = pa[1][1] = pa[1][3] = 0u;
-                l[s] = l[s] * alpha[s] + sum;
             }
             if constexpr (MODE != KD_SPLIT) {
-                const bool same = RS == 1 ? alpha[0] == 1.f : alpha[0] == 1.f && alpha[RS - 1] == 1.f;
+                bool same = true;
+#pragma unroll
+                for (int s = 0; s < SETS; s++) same = same && alpha[s][0] == 1.f && alpha[s][1] == 1.f;
                 if (!__all_sync(0xffffffffu, same)) {
 #pragma unroll
-                    for (int k = 0; k < NT; k++)
+                    for (int s = 0; s < SETS; s++)
 #pragma unroll
-                        for (int c = 0; c < OC; c++) o[k][c] *= alpha[c / 2];
+                        for (int k = 0; k < MT; k++)
+#pragma unroll
+                            for (int c = 0; c < 4; c++) o[s][k][c] *= alpha[s][c & 1];
                 }
             }
-            // ---- values: n-tile k is dimension (HD / 8) g + k
-            float d[NT][4];
+            // ---- values
+            float d[MT][4];  // f32: this tile's sums
+            if constexpr (MODE == KD_SPLIT)
 #pragma unroll
-            for (int k = 0; k < NT; k++) {
-                if constexpr (MODE == KD_SPLIT) d[k][0] = d[k][1] = d[k][2] = d[k][3] = 0.f;
-                else if constexpr (MODE == KD_ROWS8) { d[k][0] = o[k][0]; d[k][1] = o[k][1]; d[k][2] = d[k][3] = 0.f; }
-                else
-#pragma unroll
-                    for (int c = 0; c < 4; c++) d[k][c] = o[k][c % OC];
-            }
+                for (int k = 0; k < MT; k++) d[k][0] = d[k][1] = d[k][2] = d[k][3] = 0.f;
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 uint32_t vs = *reinterpret_cast<const uint32_t *>(tb + 33 * HD + ((t * G + g * G / 8) * 2 + u) * 4);
@@ -353,7 +432,7 @@ __global__ void __launch_bounds__(kd_warps(HD) * 32, KD_CTAS) k_kv4_attn_few(Kv4
                 }
 #pragma unroll
                 for (int x = 0; x < HD / 64; x++) {
-                    // pairs along the positions: byte b of e: dimension 2 b of (0, 2); of od: dimension 2 b + 1
+                    // pairs along the positions: byte b of e..: dimension 2 b, of o..: 2 b + 1; (0, 2) and (1, 3) of the quad
                     uint32_t e02[4], o02[4], e13[4], o13[4];
                     e2m1x8_to_h2((w[0][x] & 0x0F0F0F0Fu) | ((w[2][x] << 4) & 0xF0F0F0F0u), e02);
                     e2m1x8_to_h2(((w[0][x] >> 4) & 0x0F0F0F0Fu) | (w[2][x] & 0xF0F0F0F0u), o02);
@@ -361,120 +440,132 @@ __global__ void __launch_bounds__(kd_warps(HD) * 32, KD_CTAS) k_kv4_attn_few(Kv4
                     e2m1x8_to_h2(((w[1][x] >> 4) & 0x0F0F0F0Fu) | (w[3][x] & 0xF0F0F0F0u), o13);
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        mma_16816(d[8 * x + 2 * k], pa[u], hmul2_u32(e02[k], f02), hmul2_u32(e13[k], f13));
-                        mma_16816(d[8 * x + 2 * k + 1], pa[u], hmul2_u32(o02[k], f02), hmul2_u32(o13[k], f13));
+                        const uint32_t a0 = hmul2_u32(e02[k], f02), a1 = hmul2_u32(o02[k], f02);
+                        const uint32_t a2 = hmul2_u32(e13[k], f13), a3 = hmul2_u32(o13[k], f13);
+                        if constexpr (MODE == KD_SPLIT) {
+                            mma4(d[4 * x + k], a0, a1, a2, a3, pb[0][u][0], pb[0][u][1]);
+                            mma4(d[4 * x + k], a0, a1, a2, a3, pb[0][u][2], pb[0][u][3]);
+                        } else {
+#pragma unroll
+                            for (int s = 0; s < SETS; s++) mma4(o[s][4 * x + k], a0, a1, a2, a3, pb[s][u][0], pb[s][u][1]);
+                        }
                     }
                 }
             }
+            if constexpr (MODE == KD_SPLIT)
 #pragma unroll
-            for (int k = 0; k < NT; k++) {
-                if constexpr (MODE == KD_SPLIT) {
-                    o[k][0] = fmaf(o[k][0], alpha[0], d[k][0] + d[k][2]);
-                    o[k][1] = fmaf(o[k][1], alpha[0], d[k][1] + d[k][3]);
-                } else {
+                for (int k = 0; k < MT; k++)
 #pragma unroll
-                    for (int c = 0; c < OC; c++) o[k][c] = d[k][c];
-                }
-            }
+                    for (int c = 0; c < 4; c++) o[0][k][c] = fmaf(o[0][k][c], alpha[0][c & 1], d[k][c]);
             __syncwarp();  // the stage is read: the next issue may fill it
         }
 
-        // ---- the warps' results joined in shared memory
+        // ---- the warps' results joined in shared memory, each in its own drained ring: m, l, then rows of HD + 4
+        constexpr int RS = HD + 4, WS = KD_NST * TB / 4;  // floats from row to row, from warp to warp
+        static_assert(ROWS * (RS + 2) <= WS, "a warp's result fits its ring");
+        static_assert(KD_MAX_CUT * ROWS * 2 * 4 <= KD_WARPS_SHORT * KD_NST * TB, "the factors of a joined unit fit the rings");
+        float *comb = reinterpret_cast<float *>(ring);
 #pragma unroll
-        for (int s = 0; s < RS; s++) {
-            l[s] += __shfl_xor_sync(0xffffffffu, l[s], 1);
-            l[s] += __shfl_xor_sync(0xffffffffu, l[s], 2);
-            float *dst = comb + (g + 8 * s) * (HD + 2);
-            if (t == 0) {
-                dst[0] = m[s];
-                dst[1] = l[s];
+        for (int s = 0; s < SETS; s++)
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                const int r = 8 * s + 2 * t + c;
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) l[s][c] += __shfl_xor_sync(0xffffffffu, l[s][c], x);
+                if (g == 0) {
+                    comb[r] = m[s][c];
+                    comb[ROWS + r] = l[s][c];
+                }
+#pragma unroll
+                for (int k = 0; k < MT; k += 2)
+                    *reinterpret_cast<float4 *>(comb + 2 * ROWS + r * RS + 2 * MT * g + 2 * k) =
+                        make_float4(o[s][k][c], o[s][k][2 + c], o[s][k + 1][c], o[s][k + 1][2 + c]);
             }
-            // D columns 2 t, 2 t + 1 of n-tile k are the lanes g' = 2 t, 2 t + 1 of the B operand: dimensions (HD / 8) g' + k
-#pragma unroll
-            for (int k = 0; k < NT; k++)
-#pragma unroll
-                for (int c = 0; c < 2; c++) dst[2 + (2 * t + c) * NT + k] = o[k][2 * s + c];
-        }
         __syncthreads();
-        const bool whole = nt == q.tiles;
-        const long long unit0 = cur - ta;  // the line's first and last tile of this (sequence, head, group)
+        const bool whole = ncut == 1;
         const float *all = reinterpret_cast<const float *>(smem);
-        float *part = a.parts + ((size_t)b * 2 + (cur == begin ? 0 : 1)) * kv4_part_floats(ROWS, HD);
-        for (int i = tid; i < ROWS * HD; i += KD_THREADS) {
+        constexpr int PF = kv4_part_floats(ROWS, HD);
+        float *parts = a.parts + (size_t)(s_slot + hr * ncut) * PF, *part = parts + (size_t)cut * PF;  // the unit's, this piece's
+        for (int i = tid * 4; i < ROWS * HD; i += KD_THREADS * 4) {
             const int r = i / HD, dd = i - r * HD;
+            const int row = rg * ROWS + r, j = row / a.gq, h = kh * a.gq + row - j * a.gq;
+            if (j >= q.nq) continue;
             float M = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < KD_WARPS; w++) M = fmaxf(M, all[w * COMB + r * (HD + 2)]);
+            for (int w = 0; w < KD_WARPS; w++) M = fmaxf(M, all[w * WS + r]);
             const float mm = M == -INFINITY ? 0.f : M;
-            float L = 0.f, acc = 0.f;
+            float L = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int w = 0; w < KD_WARPS; w++) {
-                const float *src = all + w * COMB + r * (HD + 2);
-                const float e = ex2(src[0] - mm);
-                L += src[1] * e;
-                acc += src[2 + dd] * e;
+                const float e = ex2(all[w * WS + r] - mm);
+                const float4 v = *reinterpret_cast<const float4 *>(all + w * WS + 2 * ROWS + r * RS + dd);
+                L += all[w * WS + ROWS + r] * e;
+                acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
             }
-            const int row = rg * ROWS + r, j = row / a.gq, h = kh * a.gq + row - j * a.gq;
             if (!whole) {
-                part[2 * ROWS + i] = acc;
+                *reinterpret_cast<float4 *>(part + 2 * ROWS + i) = acc;
                 if (dd == 0) {
-                    part[2 * r] = M;
-                    part[2 * r + 1] = L;
+                    part[r] = M;
+                    part[ROWS + r] = L;
                 }
-            } else if (j < q.nq) {
+            } else {
+                float f = 1.f;
                 if (a.sinks) {
-                    const float sk = a.sinks[h] * 1.4426950408889634f, M2 = fmaxf(M, sk), m2 = M2 == -INFINITY ? 0.f : M2;
-                    const float e = ex2(M - m2);
-                    acc *= e;
-                    L = L * e + ex2(sk - m2);
+                    const float sk = a.sinks[h] * LOG2E, M2 = fmaxf(M, sk), m2 = M2 == -INFINITY ? 0.f : M2;
+                    f = ex2(M - m2);
+                    L = L * f + ex2(sk - m2);
                 }
-                static_cast<T *>(a.out)[(int64_t)(q.q0 + j) * a.ldo + (int64_t)h * HD + dd] = from_f32<T>(L > 0.f ? acc / L : 0.f);
+                f = L > 0.f ? f / L : 0.f;
+                store4f(static_cast<T *>(a.out) + (int64_t)(q.q0 + j) * a.ldo + (int64_t)h * HD + dd, a.out_wide,
+                        make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
             }
         }
         if (!whole) {
-            // the blocks that share this unit: the first one's piece is its last segment unless it begins there
-            const int f = (int)(((unit0 + 1) * nb - 1) / total), e = (int)(((unit0 + q.tiles) * nb - 1) / total);
-            const int f_slot = total * f / nb == unit0 ? 0 : 1;
-            constexpr int PF = kv4_part_floats(ROWS, HD);
             __threadfence();
             __syncthreads();
             if (tid == 0) {
                 unsigned *cnt_p = a.count + ((size_t)seq * a.c.n_kv + kh) * a.row_groups + rg;
-                const bool last = atomicAdd(cnt_p, 1u) + 1u == (unsigned)(e - f + 1);
+                const bool last = atomicAdd(cnt_p, 1u) + 1u == (unsigned)ncut;
                 if (last) *cnt_p = 0u;  // ready for the next call
                 s_last = last;
                 __threadfence();
             }
             __syncthreads();
             if (s_last) {
-                for (int i = tid; i < ROWS * HD; i += KD_THREADS) {
+                // the pieces' maxima and sums, then their factors, in the rings
+                float *mx = reinterpret_cast<float *>(smem), *ls = mx + ncut * ROWS;
+                for (int i = tid; i < ncut * ROWS; i += KD_THREADS) {
+                    const float *src = parts + (size_t)(i / ROWS) * PF + i % ROWS;
+                    mx[i] = __ldcg(src);
+                    ls[i] = __ldcg(src + ROWS);
+                }
+                __syncthreads();
+                for (int i = tid * 4; i < ROWS * HD; i += KD_THREADS * 4) {
                     const int r = i / HD, dd = i - r * HD;
                     const int row = rg * ROWS + r, j = row / a.gq, h = kh * a.gq + row - j * a.gq;
                     if (j >= q.nq) continue;
-                    const float sk = a.sinks ? a.sinks[h] * 1.4426950408889634f : -INFINITY;
-                    const float *src = a.parts + ((size_t)f * 2 + f_slot) * PF;
-                    const float *next = a.parts + (size_t)(f + 1) * 2 * PF;
-                    float M = fmaxf(sk, __ldcg(src + 2 * r));
-#pragma unroll 4
-                    for (int x = 0; x < e - f; x++) M = fmaxf(M, __ldcg(next + (size_t)x * 2 * PF + 2 * r));
+                    const float sk = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+                    float M = sk;
+                    for (int x = 0; x < ncut; x++) M = fmaxf(M, mx[x * ROWS + r]);
                     const float mm = M == -INFINITY ? 0.f : M;
-                    float w = ex2(__ldcg(src + 2 * r) - mm);
-                    float L = (a.sinks ? ex2(sk - mm) : 0.f) + __ldcg(src + 2 * r + 1) * w, acc = __ldcg(src + 2 * ROWS + i) * w;
-#pragma unroll 4
-                    for (int x = 0; x < e - f; x++) {
-                        src = next + (size_t)x * 2 * PF;
-                        w = ex2(__ldcg(src + 2 * r) - mm);
-                        L += __ldcg(src + 2 * r + 1) * w;
-                        acc += __ldcg(src + 2 * ROWS + i) * w;
+                    float L = a.sinks ? ex2(sk - mm) : 0.f;
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+                    for (int x = 0; x < ncut; x++) {
+                        const float e = ex2(mx[x * ROWS + r] - mm);
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(parts + (size_t)x * PF + 2 * ROWS + i));
+                        L += ls[x * ROWS + r] * e;
+                        acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
                     }
-                    static_cast<T *>(a.out)[(int64_t)(q.q0 + j) * a.ldo + (int64_t)h * HD + dd] = from_f32<T>(L > 0.f ? acc / L : 0.f);
+                    const float f = L > 0.f ? 1.f / L : 0.f;
+                    store4f(static_cast<T *>(a.out) + (int64_t)(q.q0 + j) * a.ldo + (int64_t)h * HD + dd, a.out_wide,
+                            make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
                 }
             }
         }
         fence_proxy_async_smem();  // the rings held the results: copies may fill them again
         __syncthreads();
-        cur += nt;
-        off += nt;
     }
     if (!ok) {  // a wait ran out: the copies still on their way, then out
         for (int i = 0; i < KD_NST; i++) {
@@ -485,24 +576,42 @@ __global__ void __launch_bounds__(kd_warps(HD) * 32, KD_CTAS) k_kv4_attn_few(Kv4
     }
 }
 
-// blocks for a call: enough to fill the GPU, and at least KD_MIN_TILES tiles each
-constexpr int KD_MIN_TILES = 16;
-static int few_blocks(const Kv4 &c, int gq, int rows, int max_q, int64_t max_kv, int window) {
+// How a call is cut: into one piece per block that fits the GPU, or, where
+// there are so many units that the pieces would be uneven, into KD_WAVES times
+// as many.  Units of a piece or less go whole, to blocks of two warps where
+// there are more of them than blocks of four fit.
+constexpr int KD_WAVES = 4;
+struct FewCut {
+    int blocks, pieces, warps;
+};
+static int few_most(int hd, int warps) { return num_sms() * (kd_warps_sm(hd) / warps); }
+static FewCut few_cut(const Kv4 &c, int gq, int rows, int max_q, int64_t max_kv, int window, int hd) {
     int64_t len = max_kv < 1 ? 1 : max_kv;
     if (window > 0 && len > (int64_t)window + max_q) len = (int64_t)window + max_q;
     const int64_t units = (int64_t)c.n_seqs * c.n_kv * ceil_div((int64_t)max_q * gq, rows);
-    const int64_t tiles = units * ((len + 31) / 32 + (window > 0 ? 1 : 0));
-    const int64_t most = (int64_t)num_sms() * KD_CTAS;
-    const int64_t want = (tiles + KD_MIN_TILES - 1) / KD_MIN_TILES;
-    return (int)(want < most ? want : most);
+    const int64_t tiles = (len + 31) / 32 + (window > 0 ? 1 : 0), most = few_most(hd, KD_WARPS_LONG);
+    FewCut f{};
+    f.pieces = (int)(units * 4 <= most ? most - units : most * KD_WAVES - (units < most ? units : most));
+    f.warps = tiles <= KD_MIN_CHUNK && units > most ? KD_WARPS_SHORT : KD_WARPS_LONG;
+    int64_t chunk = (units * tiles + f.pieces - 1) / f.pieces;
+    if (chunk < KD_MIN_CHUNK) chunk = KD_MIN_CHUNK;
+    const int64_t blocks = units * ((tiles + chunk - 1) / chunk);
+    f.blocks = (int)(blocks < (1 << 20) ? blocks : 1 << 20);
+    return f;
 }
 
-template <int HD, int MODE, typename T>
-static int launch_few(Kv4AttnArgs &a, int blocks, cudaStream_t st) {
-    TRY(ensure_smem(k_kv4_attn_few<HD, MODE, T>, kd_smem<HD>()));
-    k_kv4_attn_few<HD, MODE, T><<<blocks, kd_warps(HD) * 32, kd_smem<HD>(), st>>>(a);
+template <int HD, int MODE, typename T, int WARPS>
+static int launch_few(Kv4AttnArgs &a, const FewCut &f, cudaStream_t st) {
+    a.pieces = f.pieces;
+    TRY(ensure_smem(k_kv4_attn_few<HD, MODE, T, WARPS>, kd_smem<HD>(WARPS)));
+    k_kv4_attn_few<HD, MODE, T, WARPS><<<f.blocks, WARPS * 32, kd_smem<HD>(WARPS), st>>>(a);
     MG_CHECK_LAUNCH();
     return MG_OK;
+}
+template <int HD, int MODE, typename T>
+static int launch_few(Kv4AttnArgs &a, const FewCut &f, cudaStream_t st) {
+    return f.warps == KD_WARPS_SHORT ? launch_few<HD, MODE, T, KD_WARPS_SHORT>(a, f, st)
+                                     : launch_few<HD, MODE, T, KD_WARPS_LONG>(a, f, st);
 }
 
 // rows of the kernel for a call: 16 where 8 would need a second group and the type has no lo halves
@@ -511,13 +620,13 @@ static int few_mode(int act, int gq, int max_q) {
 }
 
 template <typename T>
-static int attn_few(Kv4AttnArgs &a, int hd, int mode, int blocks, cudaStream_t st) {
+static int attn_few(Kv4AttnArgs &a, int hd, int mode, const FewCut &f, cudaStream_t st) {
     if constexpr (sizeof(T) == 4) {
-        return hd == 64 ? launch_few<64, KD_SPLIT, T>(a, blocks, st) : launch_few<128, KD_SPLIT, T>(a, blocks, st);
+        return hd == 64 ? launch_few<64, KD_SPLIT, T>(a, f, st) : launch_few<128, KD_SPLIT, T>(a, f, st);
     } else {
         if (mode == KD_ROWS8)
-            return hd == 64 ? launch_few<64, KD_ROWS8, T>(a, blocks, st) : launch_few<128, KD_ROWS8, T>(a, blocks, st);
-        return hd == 64 ? launch_few<64, KD_ROWS16, T>(a, blocks, st) : launch_few<128, KD_ROWS16, T>(a, blocks, st);
+            return hd == 64 ? launch_few<64, KD_ROWS8, T>(a, f, st) : launch_few<128, KD_ROWS8, T>(a, f, st);
+        return hd == 64 ? launch_few<64, KD_ROWS16, T>(a, f, st) : launch_few<128, KD_ROWS16, T>(a, f, st);
     }
 }
 
@@ -533,9 +642,15 @@ static int attn_check(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv, K
 // The workspace: partial results for the most blocks of any call, so that
 // the counters behind them lie in the same place for every call, and a
 // counter per (sequence, key/value head, row group).
-constexpr int64_t attn_part_bytes(int sms) { return (int64_t)sms * KD_CTAS * 2 * kv4_part_floats(16, 128) * 4; }
+// (Pieces of cut units are at most twice FewCut::pieces: a unit of n > 1
+// pieces has more than n / 2 chunks.)
+static int64_t attn_part_bytes() {
+    const int64_t d64 = (int64_t)few_most(64, KD_WARPS_LONG) * kv4_part_floats(16, 64);
+    const int64_t d128 = (int64_t)few_most(128, KD_WARPS_LONG) * kv4_part_floats(16, 128);
+    return 2 * KD_WAVES * (d64 > d128 ? d64 : d128) * 4;
+}
 static int64_t attn_work(const Kv4 &c, int groups) {
-    return attn_part_bytes(num_sms()) + (int64_t)c.n_seqs * c.n_kv * groups * 4;
+    return attn_part_bytes() + (int64_t)c.n_seqs * c.n_kv * groups * 4;
 }
 
 }  // namespace mg
@@ -574,13 +689,16 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
     a.window = window;
     a.sinks = sinks;
     a.parts = static_cast<float *>(work);
-    a.count = reinterpret_cast<unsigned *>(static_cast<uint8_t *>(work) + attn_part_bytes(num_sms()));
+    a.count = reinterpret_cast<unsigned *>(static_cast<uint8_t *>(work) + attn_part_bytes());
+    const int64_t size = act == MG_ACT_F32 ? 4 : 2;
+    a.q_wide = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(ldq * size)) & 15) == 0;
+    a.out_wide = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * size)) & 15) == 0;
     a.err = stream_error_word();
     MG_REQUIRE(a.err, MG_ERR_OOM, "kv4_attn: no error word");
     cudaStream_t st = (cudaStream_t)stream;
     const int mode = few_mode(act, a.gq, max_q);
-    const int blocks = few_blocks(a.c, a.gq, kd_rows(mode), max_q, max_kv, window);
-    if (act == MG_ACT_F32) return attn_few<float>(a, c->head_dim, mode, blocks, st);
-    if (act == MG_ACT_F16) return attn_few<__half>(a, c->head_dim, mode, blocks, st);
-    return attn_few<__nv_bfloat16>(a, c->head_dim, mode, blocks, st);
+    const FewCut f = few_cut(a.c, a.gq, kd_rows(mode), max_q, max_kv, window, c->head_dim);
+    if (act == MG_ACT_F32) return attn_few<float>(a, c->head_dim, mode, f, st);
+    if (act == MG_ACT_F16) return attn_few<__half>(a, c->head_dim, mode, f, st);
+    return attn_few<__nv_bfloat16>(a, c->head_dim, mode, f, st);
 }

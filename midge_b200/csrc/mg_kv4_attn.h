@@ -10,16 +10,18 @@ struct Kv4AttnArgs {
     const void *q;
     void *out;
     int64_t ldq, ldo;
+    bool q_wide, out_wide;  // rows of 16-byte alignment
     const int32_t *q_start, *kv_len;
     int max_q;
     float scale;
     int window;
     const float *sinks;
-    // split work: per block two places for a partial result (kv4_part_floats
-    // each), per (sequence, key/value head, row group) a counter
+    // cut units: a place for each piece's result (kv4_part_floats) and, per
+    // (sequence, key/value head, row group), a counter of those that arrived
     float *parts;
     unsigned *count;
-    int row_groups;  // the most row groups of a sequence
+    int row_groups;   // the most row groups of a sequence
+    int pieces;       // pieces wanted of the whole call
     int *err;
 };
 

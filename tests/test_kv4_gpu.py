@@ -350,7 +350,8 @@ def test_workspace_reused_between_sizes_and_streams(torch_cuda):
     torch = torch_cuda
     rng = np.random.default_rng(8)
     dev = Dev(torch, filled(rng, [700, 20], 1, 64, 64))
-    work = torch.zeros(1 << 24, dtype=torch.uint8, device="cuda")
+    need = max(abi.check_size(abi.lib.mg_kv4_attn_work(dev.ref(), 4, n, 700)) for n in (1, 5, 50))
+    work = torch.zeros(need, dtype=torch.uint8, device="cuda")
     st = torch.cuda.Stream()
     for nq in ([1, 1], [5, 2], [1, 0], [50, 20], [1, 1]):
         qs = np.concatenate([[0], np.cumsum(nq)])
