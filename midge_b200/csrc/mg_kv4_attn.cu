@@ -50,7 +50,6 @@ enum { KD_SPLIT = 0, KD_ROWS8 = 1, KD_ROWS16 = 2 };
 __host__ __device__ constexpr int kd_rows(int mode) { return mode == KD_ROWS16 ? 16 : 8; }
 template <int HD> constexpr size_t kd_smem(int warps) { return (size_t)warps * KD_NST * kv4_tile_bytes(HD); }
 
-constexpr float LOG2E = 1.4426950408889634f;
 __device__ __forceinline__ float ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -91,35 +90,6 @@ __device__ __forceinline__ uint32_t live_bytes(uint32_t w, int p, int first, int
     if (hi < 4) w &= hi <= 0 ? 0u : (1u << (8 * hi)) - 1u;
     if (lo > 0) w &= lo >= 4 ? 0u : ~((1u << (8 * lo)) - 1u);
     return w;
-}
-
-// N consecutive elements as floats; 16 bytes at a time where the row allows
-template <int N, typename T>
-__device__ __forceinline__ void load_row(const T *src, bool wide, float x[N]) {
-    if (wide) {
-        constexpr int V = 16 / sizeof(T);
-#pragma unroll
-        for (int i = 0; i < N / V; i++) {
-            const uint4 v = reinterpret_cast<const uint4 *>(src)[i];
-            T e[V];
-            memcpy(e, &v, 16);
-#pragma unroll
-            for (int k = 0; k < V; k++) x[V * i + k] = to_f32(e[k]);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) x[i] = to_f32(src[i]);
-    }
-}
-template <typename T> __device__ __forceinline__ void store4f(T *dst, bool wide, float4 v) {
-    T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
-    if (wide) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<uint4 *>(e);
-        else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<uint2 *>(e);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) dst[i] = e[i];
-    }
 }
 
 template <int HD, int MODE, typename T, int KD_WARPS>
@@ -288,7 +258,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
             for (int c = 0; c < 2; c++) {
                 factor[s][c] = __shfl_sync(0xffffffffu, own_factor[s], (2 * t + c) * 4);
                 const int j = (rg * ROWS + 8 * s + 2 * t + c) / a.gq;
-                hi[s][c] = j < q.nq ? q.len - q.nq + j : -1;
+                hi[s][c] = j < q.nq ? q.before + j : -1;
                 m[s][c] = -INFINITY;
                 l[s][c] = 0.f;
             }
@@ -350,7 +320,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
             }
             // ---- weights
             // some row does not see some position: the last tiles, and with a window the first ones
-            const bool edge = p0 + 32 > q.len - q.nq + 1 || (a.window > 0 && p0 < q.len - a.window);
+            const bool edge = p0 + 32 > q.before + 1 || (a.window > 0 && p0 < q.before + q.nq - a.window);
             uint32_t pb[SETS][2][QR];
             float alpha[SETS][2];
 #pragma unroll
@@ -639,15 +609,21 @@ static int attn_check(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv, K
     return MG_OK;
 }
 
-// The workspace: partial results for the most blocks of any call, so that
-// the counters behind them lie in the same place for every call, and a
-// counter per (sequence, key/value head, row group).
-// (Pieces of cut units are at most twice FewCut::pieces: a unit of n > 1
-// pieces has more than n / 2 chunks.)
+// Rows of a key/value head from which the tcgen05 kernel (two tiles of 128
+// rows a block) is taken.
+constexpr int KV4_MANY_ROWS = 32;
+static bool is_many(int gq, int max_q) { return (int64_t)gq * max_q > KV4_MANY_ROWS; }
+
+// The workspace: partial results of the most pieces of any call, so that the
+// counters behind them lie in the same place for every call, and a counter
+// per (sequence, key/value head, row group).  Pieces of cut units are at most
+// twice FewCut::pieces (a unit of n > 1 pieces has more than n / 2 chunks);
+// the many-row kernel cuts only as far as all pieces fit the GPU at a time.
 static int64_t attn_part_bytes() {
     const int64_t d64 = (int64_t)few_most(64, KD_WARPS_LONG) * kv4_part_floats(16, 64);
     const int64_t d128 = (int64_t)few_most(128, KD_WARPS_LONG) * kv4_part_floats(16, 128);
-    return 2 * KD_WAVES * (d64 > d128 ? d64 : d128) * 4;
+    const int64_t few = 2 * KD_WAVES * (d64 > d128 ? d64 : d128) * 4, many = (int64_t)num_sms() * kv4_part_floats(256, 128) * 4;
+    return few > many ? few : many;
 }
 static int64_t attn_work(const Kv4 &c, int groups) {
     return attn_part_bytes() + (int64_t)c.n_seqs * c.n_kv * groups * 4;
@@ -696,6 +672,12 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
     a.err = stream_error_word();
     MG_REQUIRE(a.err, MG_ERR_OOM, "kv4_attn: no error word");
     cudaStream_t st = (cudaStream_t)stream;
+    if (is_many(a.gq, max_q)) {
+        const int row_tiles = ceil_div((int64_t)max_q * a.gq, 256);
+        int64_t len = window > 0 && max_kv > (int64_t)window + max_q ? (int64_t)window + max_q : max_kv;
+        const int cuts = kv4_many_cuts((int64_t)c->n_seqs * c->n_kv_heads * row_tiles, ceil_div(len, 128));
+        return kv4_attn_many(a, c->head_dim, act, row_tiles, cuts, st);
+    }
     const int mode = few_mode(act, a.gq, max_q);
     const FewCut f = few_cut(a.c, a.gq, kd_rows(mode), max_q, max_kv, window, c->head_dim);
     if (act == MG_ACT_F32) return attn_few<float>(a, c->head_dim, mode, f, st);

@@ -1,5 +1,7 @@
 // mg_kv4_attn.h -- arguments of the attention kernels over the 4-bit cache.
 #pragma once
+#include <string.h>
+
 #include "mg_kv4.cuh"
 
 namespace mg {
@@ -31,18 +33,54 @@ __host__ __device__ constexpr int kv4_part_floats(int rows, int hd) { return row
 
 // A sequence's share of the work.
 struct Kv4Seq {
-    int q0, nq, len, first, tile0, tiles;  // first: first position its first query sees
+    int q0, nq, len, before, first, tile0, tiles;  // before: its first query's position, first: the first it sees
     __device__ __forceinline__ void load(const Kv4AttnArgs &a, int s) {
         q0 = a.q_start[s];
-        nq = min(a.q_start[s + 1] - q0, a.max_q);
-        const int l = a.kv_len[s];
+        const int n = a.q_start[s + 1] - q0, l = a.kv_len[s];
+        nq = min(n, a.max_q);
         len = (int)min((int64_t)max(l, 0), a.c.cap);
-        first = a.window > 0 ? max(0, len - nq - a.window + 1) : 0;
+        before = len - n;
+        first = a.window > 0 ? max(0, before - a.window + 1) : 0;
         tile0 = first >> 5;
         // at least one tile where there is a query, so that its zeros are written
         tiles = nq <= 0 ? 0 : max(1, ((len + 31) >> 5) - tile0);
     }
     __device__ __forceinline__ int groups(int gq, int rows) const { return nq <= 0 ? 0 : (nq * gq + rows - 1) / rows; }
 };
+
+constexpr float LOG2E = 1.4426950408889634f;
+
+// N consecutive elements as floats; 16 bytes at a time where the row allows
+template <int N, typename T>
+__device__ __forceinline__ void load_row(const T *src, bool wide, float x[N]) {
+    if (wide) {
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < N / V; i++) {
+            const uint4 v = reinterpret_cast<const uint4 *>(src)[i];
+            T e[V];
+            memcpy(e, &v, 16);
+#pragma unroll
+            for (int k = 0; k < V; k++) x[V * i + k] = to_f32(e[k]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = to_f32(src[i]);
+    }
+}
+template <typename T> __device__ __forceinline__ void store4f(T *dst, bool wide, float4 v) {
+    T e[4] = {from_f32<T>(v.x), from_f32<T>(v.y), from_f32<T>(v.z), from_f32<T>(v.w)};
+    if (wide) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<uint4 *>(e);
+        else *reinterpret_cast<uint2 *>(dst) = *reinterpret_cast<uint2 *>(e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) dst[i] = e[i];
+    }
+}
+
+// mg_kv4_prompt.cu: blocks of 256 rows; cuts: pieces of a unit
+int kv4_many_cuts(int64_t units, int64_t blocks);
+int kv4_attn_many(const Kv4AttnArgs &a, int hd, int act, int row_tiles, int cuts, cudaStream_t st);
 
 }  // namespace mg

@@ -1,0 +1,548 @@
+// mg_kv4_prompt.cu -- attention of many new queries over the 4-bit paged
+// cache (prompt chunks, several drafted tokens) on the 5th-generation tensor
+// cores.
+//
+// A block has 256 rows ((query, head) pairs of one key/value head, two tiles
+// of 128) and walks the cache in blocks of KVB positions:
+//   warps 0-3, 4-7    softmax of tile 0 / 1, thread = row: S from TMEM, row
+//                     maximum, weights as f16 back into TMEM over S, the
+//                     products of the last block added to O in registers
+//   warps 8-14        codes -> f16 K and V tiles in 128-byte-swizzled shared
+//                     memory (cvt.f16x2.e2m1x2 and the scale: exact), once
+//                     for both tiles
+//   warp 15           one thread issues the MMAs: S = Q K^T (both from shared
+//                     memory), O_block = P V (P from TMEM)
+// The two tiles alternate: while one tile's MMAs run the other's softmax has
+// the MUFU, which bounds the kernel (16 ex2 per cycle and SM against 4096
+// multiply-adds: at head_dim 64 the exponentials take twice the MMAs' time).
+// O stays in registers in fp32 and each block's product starts from zero: the
+// tensor core truncates its running sum.  f32 rows go as f16 hi + lo, queries
+// and weights (two MMAs each, 22 bits); f16 and bf16 queries are exact in f16
+// after scaling by a power of two per row.
+#include "mg_kernels.h"
+#include "mg_kv4_attn.h"
+#include "mg_tc.cuh"
+
+namespace mg {
+
+constexpr int KP_ROWS = 256;        // rows of a block
+constexpr int KP_THREADS = 512;
+constexpr int KP_DEQ = 7;           // warps 8-14
+constexpr int KP_ERR = 42;
+constexpr int KP_REG_SOFTMAX = 200, KP_REG_OTHER = 56;
+static_assert(KP_REG_SOFTMAX + KP_REG_OTHER == 256, "two warpgroups of each out of 512 x 128 registers");
+
+template <int HD, bool SPLIT>
+struct KpCfg {
+    static constexpr int KVB = HD == 128 && SPLIT ? 64 : 128;  // positions of a block
+    static constexpr int PLANES = HD / 64;                     // 64 dimensions = 128 bytes a row
+    static constexpr int Q_HALF = PLANES * 128 * 128;          // bytes of one tile's hi (or lo) queries
+    static constexpr int Q_TILE = Q_HALF * (SPLIT ? 2 : 1);
+    static constexpr int KV_STAGE = PLANES * KVB * 128;        // bytes of a K (or V) stage
+    static constexpr int SMEM = 2 * Q_TILE + 4 * KV_STAGE + 1024;
+    static constexpr int TM_S = KVB, TM_O = HD;                // TMEM columns of a tile
+};
+
+__device__ __forceinline__ float kp_ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+// 32 consecutive columns of this thread's TMEM lane, complete on return
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float v[32]) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t v[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+// V, [position][64 dimensions] rows of 128 bytes, 128-byte swizzle, dimensions contiguous ("MN-major"): 8-position
+// groups 1024 bytes apart, planes of 64 dimensions `plane` bytes apart
+__device__ __forceinline__ uint64_t desc_v(uint32_t addr, uint32_t plane) {
+    return (uint64_t)((addr >> 4) & 0x3FFF) | ((uint64_t)(plane >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
+           ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
+}
+__device__ __forceinline__ uint32_t kp_h2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&h);
+}
+__device__ __forceinline__ void kp_split(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    hi = *reinterpret_cast<const uint32_t *>(&h);
+    lo = kp_h2(a - f.x, b - f.y);
+}
+__device__ __forceinline__ uint32_t kp_scale(uint32_t w, int b) { return __byte_perm(w, 0u, (b << 12) | (b << 4) | 0x404); }
+__device__ __forceinline__ uint4 kp_eight(uint32_t codes, uint32_t f) {  // eight codes -> f16
+    uint32_t h[4];
+    e2m1x8_to_h2(codes, h);
+    return make_uint4(hmul2_u32(h[0], f), hmul2_u32(h[1], f), hmul2_u32(h[2], f), hmul2_u32(h[3], f));
+}
+
+// One warp's 16-byte pieces of a block's keys or values, a phase at a time.
+// KVB / 32 cache tiles have HD / 32 pieces each of keys, and of values.
+template <int HD, int KVB>
+struct KpPieces {
+    static constexpr int PER = HD / 32, N = KVB / 32 * PER, MINE = (N + KP_DEQ - 1) / KP_DEQ;
+    uint4 raw[MINE];
+    uint32_t sc[MINE];
+};
+
+template <int HD, bool SPLIT, typename T>
+__global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, int row_tiles, int cuts) {
+    using C = KpCfg<HD, SPLIT>;
+    constexpr int KVB = C::KVB, TB = kv4_tile_bytes(HD), G = HD / 32;
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
+    uint8_t *sq = base, *sk = base + 2 * C::Q_TILE, *sv = sk + 2 * C::KV_STAGE;
+    __shared__ uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full;
+    __shared__ uint32_t tmem_base;
+    __shared__ int s_last;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    // ---- the unit: later rows first, they see the most; pieces of a unit side by side
+    int u = blockIdx.x;
+    const int cut = u % cuts;
+    u /= cuts;
+    const int kh = u % a.c.n_kv;
+    u /= a.c.n_kv;
+    const int seq = u % a.c.n_seqs, rt = row_tiles - 1 - u / a.c.n_seqs;
+    Kv4Seq q;
+    q.load(a, seq);
+    const int rows = q.nq * a.gq - rt * KP_ROWS;  // rows from this block's first to the sequence's last
+    if (rows <= 0) return;
+    const int before = q.before;                  // position of query 0
+    // tile i's last row's position, and the blocks of positions it needs from start on
+    const int j_first = rt * KP_ROWS / a.gq;
+    const int start = a.window > 0 ? max(0, before + j_first - a.window + 1) & ~31 : 0;
+    int nb[2], first_p[2], last_p[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int r0 = rt * KP_ROWS + 128 * i, r1 = min(r0 + 127, q.nq * a.gq - 1);
+        first_p[i] = before + r0 / a.gq;
+        last_p[i] = before + r1 / a.gq;
+        nb[i] = 128 * i < rows ? max(0, (last_p[i] + 1 - start + KVB - 1) / KVB) : 0;
+    }
+    const int all_blocks = max(nb[0], nb[1]);
+    const int ncut = max(1, min(cuts, all_blocks));
+    if (cut >= ncut) return;
+    const int blk0 = (int)((long long)all_blocks * cut / ncut), blk1 = (int)((long long)all_blocks * (cut + 1) / ncut);
+    const int nblk = blk1 - blk0;
+#pragma unroll
+    for (int i = 0; i < 2; i++) nb[i] = max(0, min(nb[i], blk1) - blk0);
+    const int pos0 = start + blk0 * KVB;  // of this piece
+
+    if (tid == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&k_full[i], KP_DEQ);
+            mbar_init(&v_full[i], KP_DEQ);
+            mbar_init(&k_empty[i], 1);
+            mbar_init(&v_empty[i], 1);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 4);
+            mbar_init(&o_full[i], 1);
+        }
+        mbar_init(&q_full, 8);
+        fence_mbar_init();
+    }
+    if (warp == 15) tmem_alloc(&tmem_base, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = tmem_base;
+    bool ok = true;
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REG_OTHER));
+        if (warp == 15) {
+            // ------------------------------------------------ MMA issuer
+            if (lane == 0 && nblk > 0) {
+                constexpr uint32_t id_s = umma_idesc_f16(128, KVB);
+                constexpr uint32_t id_o = umma_idesc_f16(128, HD) | (1u << 16);  // B with its N contiguous
+                auto scores = [&](int i, int b) {
+                    const uint32_t qa = smem_u32(sq + i * C::Q_TILE), kb = smem_u32(sk + (b & 1) * C::KV_STAGE);
+#pragma unroll
+                    for (int k = 0; k < HD / 16; k++) {
+                        const uint32_t ko = (k >> 2) * (KVB * 128) + (k & 3) * 32, qo = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                        tc_mma_f16(tmem + i * C::TM_S, umma_desc_sw128(qa + qo), umma_desc_sw128(kb + ko), id_s, k > 0);
+                        if (SPLIT)
+                            tc_mma_f16(tmem + i * C::TM_S, umma_desc_sw128(qa + C::Q_HALF + qo), umma_desc_sw128(kb + ko), id_s, 1u);
+                    }
+                    tc_commit(&s_full[i]);
+                };
+                auto products = [&](int i, int b) {
+                    const uint32_t vb = smem_u32(sv + (b & 1) * C::KV_STAGE), o = tmem + 2 * C::TM_S + i * C::TM_O;
+#pragma unroll
+                    for (int k = 0; k < KVB / 16; k++) {
+                        // weights of 32 positions: 16 columns of hi, then 16 of lo
+                        const uint32_t p = tmem + i * C::TM_S + (k >> 1) * 32 + (k & 1) * 8;
+                        const uint64_t d = desc_v(vb + k * 2048, KVB * 128);
+                        tc_mma_f16_ts(o, p, d, id_o, k > 0);
+                        if (SPLIT) tc_mma_f16_ts(o, p + 16, d, id_o, 1u);
+                    }
+                };
+                ok = mbar_wait(&q_full, 0) && mbar_wait(&k_full[0], 0);
+                tc_fence_after();
+                if (ok) {
+                    for (int i = 0; i < 2; i++)
+                        if (nb[i] > 0) scores(i, 0);
+                    tc_commit(&k_empty[0]);
+                }
+                for (int b = 0; b < nblk && ok; b++) {
+                    const uint32_t par = (b >> 1) & 1, par1 = ((b + 1) >> 1) & 1;
+                    ok = mbar_wait(&v_full[b & 1], par);
+                    if (ok && b + 1 < nblk) ok = mbar_wait(&k_full[(b + 1) & 1], par1);
+                    for (int i = 0; i < 2 && ok; i++) {
+                        if (b >= nb[i]) continue;
+                        ok = mbar_wait(&p_full[i], b & 1);
+                        if (!ok) break;
+                        tc_fence_after();
+                        products(i, b);
+                        if (b + 1 < nb[i]) scores(i, b + 1);
+                        else tc_commit(&o_full[i]);
+                    }
+                    tc_commit(&v_empty[b & 1]);
+                    if (b + 1 < nblk) tc_commit(&k_empty[(b + 1) & 1]);
+                }
+                if (!ok) atomicExch(a.err, KP_ERR);
+            }
+        } else {
+            // ------------------------------------------------ codes -> f16
+            using P = KpPieces<HD, KVB>;
+            const int w = warp - 8, g = lane >> 2, t = lane & 3;
+            const int ntile = (int)((a.c.cap - 1) >> 5);
+            const uint8_t *addr = nullptr;  // lane i: the cache tile addr_base + i of this piece
+            int addr_base = -64;
+            P kp, vp;
+            auto load = [&](P &p, int b, bool key) {
+                if (b >= nblk) return;
+                constexpr int TILES = KVB / 32;
+                if (b * TILES >= addr_base + 32) {
+                    addr_base = b * TILES;
+                    addr = a.c.tile(seq, kh, min((pos0 >> 5) + addr_base + lane, ntile), TB);
+                }
+#pragma unroll
+                for (int x = 0; x < P::MINE; x++) {
+                    const int y = w + x * KP_DEQ;
+                    if (y >= P::N) break;
+                    const uint8_t *tb = reinterpret_cast<const uint8_t *>(__shfl_sync(
+                        0xffffffffu, reinterpret_cast<uint64_t>(addr), b * TILES + y / P::PER - addr_base));
+                    const int pc = y % P::PER, u = HD == 64 ? pc : pc >> 1;
+                    p.raw[x] = __ldg(reinterpret_cast<const uint4 *>(tb + (key ? 0 : 16 * HD) + pc * 512 + lane * 16));
+                    p.sc[x] = __ldg(reinterpret_cast<const uint32_t *>(
+                        tb + (key ? 32 * HD + (g * G + t * G / 4) * 4 : 33 * HD + ((t * G + g * G / 8) * 2 + u) * 4)));
+                }
+            };
+            auto put = [&](uint8_t *stage, int row, int chunk, uint4 v) {
+                *reinterpret_cast<uint4 *>(stage + (chunk >> 3) * (KVB * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4)) = v;
+            };
+            load(kp, 0, true);
+            load(vp, 0, false);
+            for (int b = 0; b < nblk && ok; b++) {
+                const int st = b & 1;
+                if (b >= 2) ok = mbar_wait(&k_empty[st], ((b >> 1) - 1) & 1);
+                if (!ok) break;
+                uint8_t *ks = sk + st * C::KV_STAGE, *vs = sv + st * C::KV_STAGE;
+#pragma unroll
+                for (int x = 0; x < P::MINE; x++) {
+                    const int y = w + x * KP_DEQ;
+                    if (y >= P::N) break;
+                    const int row0 = y / P::PER * 32, pc = y % P::PER;
+                    const uint32_t *cw = reinterpret_cast<const uint32_t *>(&kp.raw[x]);
+                    if constexpr (HD == 64) {  // words: position 2 g + (0, 1) x 16 dimensions
+                        const int odd = g & 1;  // odd lanes take the other half first: no two lanes on a bank
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            const uint32_t f = kp_scale(kp.sc[x], 2 * pc + j);
+                            const int row = row0 + 16 * pc + 2 * g + j;
+                            const uint32_t c0 = odd ? cw[2 * j + 1] : cw[2 * j], c1 = odd ? cw[2 * j] : cw[2 * j + 1];
+                            put(ks, row, 2 * t + odd, kp_eight(c0, f));
+                            put(ks, row, 2 * t + (odd ^ 1), kp_eight(c1, f));
+                        }
+                    } else {  // words: 32 dimensions of position 2 g + j
+                        const int far = t >> 1;
+                        const uint32_t f = __byte_perm(kp.sc[x], 0u, (pc << 12) | (pc << 4) | 0x404);
+                        const int row = row0 + 16 * (pc >> 1) + 2 * g + (pc & 1);
+#pragma unroll
+                        for (int k = 0; k < 4; k += 2) {
+                            const uint32_t c0 = far ? cw[k + 1] : cw[k], c1 = far ? cw[k] : cw[k + 1];
+                            put(ks, row, 4 * t + k + far, kp_eight(c0, f));
+                            put(ks, row, 4 * t + k + (far ^ 1), kp_eight(c1, f));
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[st]);
+                load(kp, b + 1, true);
+
+                if (b >= 2) ok = mbar_wait(&v_empty[st], ((b >> 1) - 1) & 1);
+                if (!ok) break;
+                const int bp = pos0 + b * KVB;
+#pragma unroll
+                for (int x = 0; x < P::MINE; x++) {
+                    const int y = w + x * KP_DEQ;
+                    if (y >= P::N) break;
+                    const int row0 = y / P::PER * 32, pc = y % P::PER, u = HD == 64 ? pc : pc >> 1;
+                    const uint32_t *cw = reinterpret_cast<const uint32_t *>(&vp.raw[x]);
+                    uint32_t sc = vp.sc[x];
+                    {   // positions that nobody wrote: any byte may stand there, a NaN scale among them
+                        const int p = bp + row0 + 16 * u + 4 * t, above = q.len - p, below = q.first - p;
+                        if (above < 4) sc &= above <= 0 ? 0u : (1u << (8 * above)) - 1u;
+                        if (below > 0) sc &= below >= 4 ? 0u : ~((1u << (8 * below)) - 1u);
+                    }
+                    const int far = t >> 1;
+                    if constexpr (HD == 64) {  // words: 8 dimensions of position 4 t + i
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const int ii = i ^ (far << 1);
+                            const uint32_t c = far ? cw[i ^ 2] : cw[i];
+                            put(vs, row0 + 16 * u + 4 * t + ii, g, kp_eight(c, __byte_perm(sc, 0u, (ii << 12) | (ii << 4) | 0x404)));
+                        }
+                    } else {  // words: 16 dimensions of position 4 t + c, then of 4 t + c + 2
+#pragma unroll
+                        for (int s = 0; s < 2; s++) {
+                            const int i = (pc & 1) + 2 * s;
+                            const uint32_t f = __byte_perm(sc, 0u, (i << 12) | (i << 4) | 0x404);
+                            const int row = row0 + 16 * u + 4 * t + i;
+                            const uint32_t c0 = far ? cw[2 * s + 1] : cw[2 * s], c1 = far ? cw[2 * s] : cw[2 * s + 1];
+                            put(vs, row, 2 * g + far, kp_eight(c0, f));
+                            put(vs, row, 2 * g + (far ^ 1), kp_eight(c1, f));
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[st]);
+                load(vp, b + 1, false);
+            }
+            if (!ok && lane == 0) atomicExch(a.err, KP_ERR);
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_REG_SOFTMAX));
+        // ---------------------------------------------------- softmax, thread = row
+        const int i = warp >> 2, r = tid & 127, row = rt * KP_ROWS + 128 * i + r;
+        const int j = row / a.gq, h = kh * a.gq + row - j * a.gq;
+        const bool live = j < q.nq;
+        const int hi = live ? before + j : -1, lo = a.window > 0 ? hi - a.window + 1 : 0;
+        float factor;
+        {   // the row's queries, scaled to below 2 by a power of two, into the swizzled tile; the scale's sign goes with them
+            const T *src = static_cast<const T *>(a.q) + (int64_t)(q.q0 + j) * a.ldq + (int64_t)h * HD;
+            float top = 0.f;
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) {
+                float x[16];
+                if (live) load_row<16>(src + c, a.q_wide, x);
+#pragma unroll
+                for (int k = 0; k < 16; k++) top = live ? fmaxf(top, fabsf(x[k])) : 0.f;
+            }
+            const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+            const float down = __uint_as_float((254u - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
+            factor = fabsf(a.scale) * LOG2E * __uint_as_float(e << 23);
+            uint8_t *dst = sq + i * C::Q_TILE + r * 128;
+#pragma unroll 1
+            for (int c = 0; c < HD / 16; c++) {
+                float x[16];
+                if (live) load_row<16>(src + c * 16, a.q_wide, x);
+#pragma unroll
+                for (int half = 0; half < 2; half++) {
+                    uint32_t vh[4], vl[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const float x0 = live ? x[8 * half + 2 * k] * down : 0.f, x1 = live ? x[8 * half + 2 * k + 1] * down : 0.f;
+                        if (SPLIT) kp_split(x0, x1, vh[k], vl[k]);
+                        else vh[k] = kp_h2(x0, x1);
+                    }
+                    const int chunk = 2 * c + half;
+                    uint8_t *at = dst + (chunk >> 3) * (128 * 128) + (((chunk & 7) ^ (r & 7)) << 4);
+                    *reinterpret_cast<uint4 *>(at) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
+                    if (SPLIT) *reinterpret_cast<uint4 *>(at + C::Q_HALF) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full);
+        }
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t ts = tmem + lanes + i * C::TM_S, to = tmem + lanes + 2 * C::TM_S + i * C::TM_O;
+        float m = -INFINITY, l = 0.f, alpha = 1.f;
+        float o[HD];
+#pragma unroll
+        for (int k = 0; k < HD; k++) o[k] = 0.f;
+        auto add_products = [&]() {  // the last block's, with the factor that its maximum gave
+#pragma unroll
+            for (int c = 0; c < HD / 32; c++) {
+                float v[32];
+                tmem_ld32(to + 32 * c, v);
+#pragma unroll
+                for (int k = 0; k < 32; k++) o[32 * c + k] = fmaf(o[32 * c + k], alpha, v[k]);
+            }
+        };
+        for (int b = 0; b < nb[i]; b++) {
+            ok = mbar_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
+            if (!ok) break;
+            tc_fence_after();
+            if (b > 0) add_products();
+            const int bp = pos0 + b * KVB;
+            const bool edge = bp + KVB - 1 > first_p[i] || (a.window > 0 && bp < last_p[i] - a.window + 1);
+            const int c_lo = max(lo - bp, 0);
+            const unsigned span = (unsigned)max(hi - bp - c_lo, -1) + 1u;  // columns c_lo .. c_lo + span - 1 are seen
+            float top = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < KVB / 32; c++) {
+                float v[32];
+                tmem_ld32(ts + 32 * c, v);
+                if (edge) {
+#pragma unroll
+                    for (int k = 0; k < 32; k++) v[k] = (unsigned)(32 * c + k - c_lo) < span ? v[k] : -INFINITY;
+                }
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) top = max3(top, v[k], v[k + 1]);
+            }
+            const float mn = top == -INFINITY ? m : fmaxf(m, top * factor), mm = mn == -INFINITY ? 0.f : mn;
+            alpha = kp_ex2(m - mm);
+            m = mn;
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int c = 0; c < KVB / 32; c++) {
+                float v[32];
+                tmem_ld32(ts + 32 * c, v);
+                uint32_t w[32];
+#pragma unroll
+                for (int k = 0; k < 32; k += 2) {
+                    float e0 = kp_ex2(fmaf(v[k], factor, -mm)), e1 = kp_ex2(fmaf(v[k + 1], factor, -mm));
+                    if (edge) {
+                        e0 = (unsigned)(32 * c + k - c_lo) < span ? e0 : 0.f;
+                        e1 = (unsigned)(32 * c + k + 1 - c_lo) < span ? e1 : 0.f;
+                    }
+                    s0 += e0;
+                    s1 += e1;
+                    if (SPLIT) kp_split(e0, e1, w[k / 2], w[16 + k / 2]);
+                    else w[k / 2] = kp_h2(e0, e1);
+                }
+                if (SPLIT) tmem_st32(ts + 32 * c, w);
+                else tmem_st16(ts + 32 * c, w);
+            }
+            l = fmaf(l, alpha, s0 + s1);
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[i]);
+        }
+        if (nb[i] > 0 && ok) {
+            ok = mbar_wait(&o_full[i], 0);
+            tc_fence_after();
+            if (ok) add_products();
+        }
+        if (!ok && lane == 0) atomicExch(a.err, KP_ERR);
+        // ---- the row's result, or this piece's part of it
+        const float sk2 = a.sinks && live ? a.sinks[h] * LOG2E : -INFINITY;
+        if (ncut == 1) {
+            if (live) {
+                const float M = fmaxf(m, sk2), mm = M == -INFINITY ? 0.f : M, e = kp_ex2(m - mm);
+                const float L = l * e + (a.sinks ? kp_ex2(sk2 - mm) : 0.f), f = L > 0.f ? e / L : 0.f;
+                T *dst = static_cast<T *>(a.out) + (int64_t)(q.q0 + j) * a.ldo + (int64_t)h * HD;
+#pragma unroll
+                for (int k = 0; k < HD; k += 4)
+                    store4f(dst + k, a.out_wide, make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f));
+            }
+        } else {
+            const size_t unit = ((size_t)seq * a.c.n_kv + kh) * row_tiles + rt;
+            constexpr size_t PF = kv4_part_floats(KP_ROWS, HD);
+            float *parts = a.parts + unit * cuts * PF, *part = parts + (size_t)cut * PF;
+            const int rr = 128 * i + r;
+            part[rr] = m;
+            part[KP_ROWS + rr] = l;
+#pragma unroll
+            for (int k = 0; k < HD; k += 4)
+                *reinterpret_cast<float4 *>(part + 2 * KP_ROWS + (size_t)rr * HD + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
+            __threadfence();
+            named_bar_sync(1, 256);
+            if (tid == 0) {
+                unsigned *cnt = a.count + ((size_t)seq * a.c.n_kv + kh) * a.row_groups + rt;
+                const bool last = atomicAdd(cnt, 1u) + 1u == (unsigned)ncut;
+                if (last) *cnt = 0u;
+                s_last = last;
+                __threadfence();
+            }
+            named_bar_sync(1, 256);
+            if (s_last) {
+                // thread = 4 dimensions of a row
+                for (int x = tid * 4; x < min(rows, KP_ROWS) * HD; x += 256 * 4) {
+                    const int r2 = x / HD, d = x - r2 * HD, row2 = rt * KP_ROWS + r2, j2 = row2 / a.gq;
+                    const int h2 = kh * a.gq + row2 - j2 * a.gq;
+                    const float sk = a.sinks ? a.sinks[h2] * LOG2E : -INFINITY;
+                    float M = sk;
+#pragma unroll 4
+                    for (int c = 0; c < ncut; c++) M = fmaxf(M, __ldcg(parts + c * PF + r2));
+                    const float mm = M == -INFINITY ? 0.f : M;
+                    float L = a.sinks ? kp_ex2(sk - mm) : 0.f;
+                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+                    for (int c = 0; c < ncut; c++) {
+                        const float e = kp_ex2(__ldcg(parts + c * PF + r2) - mm);
+                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(parts + c * PF + 2 * KP_ROWS + x));
+                        L += __ldcg(parts + c * PF + KP_ROWS + r2) * e;
+                        acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
+                    }
+                    const float f = L > 0.f ? 1.f / L : 0.f;
+                    store4f(static_cast<T *>(a.out) + (int64_t)(q.q0 + j2) * a.ldo + (int64_t)h2 * HD + d, a.out_wide,
+                            make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 15) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+// pieces of a unit: as many as still fit the GPU at a time, one where the units fill it
+int kv4_many_cuts(int64_t units, int64_t blocks) {
+    const int64_t c = num_sms() / (units > 0 ? units : 1);
+    return (int)(c < 1 ? 1 : (c > blocks ? (blocks < 1 ? 1 : blocks) : c));
+}
+
+template <int HD, bool SPLIT, typename T>
+static int launch_many(const Kv4AttnArgs &a, int row_tiles, int cuts, cudaStream_t st) {
+    constexpr int smem = KpCfg<HD, SPLIT>::SMEM;
+    TRY(ensure_smem(k_kv4_attn_many<HD, SPLIT, T>, smem));
+    const int64_t blocks = (int64_t)row_tiles * a.c.n_seqs * a.c.n_kv * cuts;
+    MG_REQUIRE(blocks < (1LL << 31), MG_ERR_ARG, "kv4_attn: too many rows");
+    k_kv4_attn_many<HD, SPLIT, T><<<(unsigned)blocks, KP_THREADS, smem, st>>>(a, row_tiles, cuts);
+    MG_CHECK_LAUNCH();
+    return MG_OK;
+}
+
+int kv4_attn_many(const Kv4AttnArgs &a, int hd, int act, int row_tiles, int cuts, cudaStream_t st) {
+    if (act == MG_ACT_F32)
+        return hd == 64 ? launch_many<64, true, float>(a, row_tiles, cuts, st) : launch_many<128, true, float>(a, row_tiles, cuts, st);
+    if (act == MG_ACT_F16)
+        return hd == 64 ? launch_many<64, false, __half>(a, row_tiles, cuts, st) : launch_many<128, false, __half>(a, row_tiles, cuts, st);
+    return hd == 64 ? launch_many<64, false, __nv_bfloat16>(a, row_tiles, cuts, st)
+                    : launch_many<128, false, __nv_bfloat16>(a, row_tiles, cuts, st);
+}
+
+}  // namespace mg
