@@ -19,6 +19,8 @@
 // tensor core truncates its running sum.  f32 rows go as f16 hi + lo, queries
 // and weights (two MMAs each, 22 bits); f16 and bf16 queries are exact in f16
 // after scaling by a power of two per row.
+#include <type_traits>
+
 #include "mg_kernels.h"
 #include "mg_kv4_attn.h"
 #include "mg_tc.cuh"
@@ -29,7 +31,7 @@ constexpr int KP_ROWS = 256;        // rows of a block
 constexpr int KP_THREADS = 512;
 constexpr int KP_DEQ = 7;           // warps 8-14
 constexpr int KP_ERR = 42;
-constexpr int KP_REG_SOFTMAX = 200, KP_REG_OTHER = 56;
+constexpr int KP_REG_SOFTMAX = 192, KP_REG_OTHER = 64;
 static_assert(KP_REG_SOFTMAX + KP_REG_OTHER == 256, "two warpgroups of each out of 512 x 128 registers");
 
 template <int HD, bool SPLIT>
@@ -41,6 +43,7 @@ struct KpCfg {
     static constexpr int KV_STAGE = PLANES * KVB * 128;        // bytes of a K (or V) stage
     static constexpr int SMEM = 2 * Q_TILE + 4 * KV_STAGE + 1024;
     static constexpr int TM_S = KVB, TM_O = HD;                // TMEM columns of a tile
+    static constexpr int CH = 16;                              // score columns a thread has at a time (two of them)
 };
 
 __device__ __forceinline__ float kp_ex2(float x) {
@@ -53,20 +56,28 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// 32 consecutive columns of this thread's TMEM lane, complete on return
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, float v[32]) {
-    uint32_t r[32];
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];\n tcgen05.wait::ld.sync.aligned;"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr)
-        : "memory");
-#pragma unroll
-    for (int i = 0; i < 32; i++) v[i] = __uint_as_float(r[i]);
+// N (16 or 32) consecutive columns of this thread's TMEM lane: the load's start, and the wait that makes r readable
+#define KP_R16(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), \
+                     "=r"(r[o + 6]), "=r"(r[o + 7]), "=r"(r[o + 8]), "=r"(r[o + 9]), "=r"(r[o + 10]), "=r"(r[o + 11]), \
+                     "=r"(r[o + 12]), "=r"(r[o + 13]), "=r"(r[o + 14]), "=r"(r[o + 15])
+#define KP_RW16(r, o) "+r"(r[o]), "+r"(r[o + 1]), "+r"(r[o + 2]), "+r"(r[o + 3]), "+r"(r[o + 4]), "+r"(r[o + 5]), \
+                      "+r"(r[o + 6]), "+r"(r[o + 7]), "+r"(r[o + 8]), "+r"(r[o + 9]), "+r"(r[o + 10]), "+r"(r[o + 11]), \
+                      "+r"(r[o + 12]), "+r"(r[o + 13]), "+r"(r[o + 14]), "+r"(r[o + 15])
+template <int N>
+__device__ __forceinline__ void tmem_ld_start(uint32_t taddr, uint32_t (&r)[N]) {
+    if constexpr (N == 16) {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                     : KP_R16(r, 0) : "r"(taddr) : "memory");
+    } else {
+        asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
+                     "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                     : KP_R16(r, 0), KP_R16(r, 16) : "r"(taddr) : "memory");
+    }
+}
+template <int N>
+__device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[N]) {
+    if constexpr (N == 16) asm volatile("tcgen05.wait::ld.sync.aligned;" : KP_RW16(r, 0)::"memory");
+    else asm volatile("tcgen05.wait::ld.sync.aligned;" : KP_RW16(r, 0), KP_RW16(r, 16)::"memory");
 }
 __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t v[16]) {
     asm volatile(
@@ -74,6 +85,43 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t v[16]) 
         "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
         "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t v[8]) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(v[0]),
+                 "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                 : "memory");
+}
+template <int N>
+__device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[N]) {
+    if constexpr (N == 8) tmem_st8(taddr, v);
+    else if constexpr (N == 16) tmem_st16(taddr, v);
+    else tmem_st32(taddr, v);
+}
+// mbar_wait whose polls sleep in the hardware for up to a microsecond each: the other roles need the issue slots
+__device__ __forceinline__ bool kp_wait(uint64_t *bar, uint32_t parity) {
+    for (uint32_t i = 0; i < MBAR_POLLS; i++) {
+        uint32_t done;
+        asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "r"(1000u) : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+// MMAs and commits issued by one elected lane of a converged warp: descriptors stay in uniform registers (from one
+// divergent lane each MMA cost some 100 cycles of moves)
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile("{\n .reg .pred p, e;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+                 " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(idesc),
+                 "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint64_t *bar) {
+    asm volatile("{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+                 " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar)) : "memory");
 }
 // V, [position][64 dimensions] rows of 128 bytes, 128-byte swizzle, dimensions contiguous ("MN-major"): 8-position
 // groups 1024 bytes apart, planes of 64 dimensions `plane` bytes apart
@@ -107,6 +155,47 @@ struct KpPieces {
     uint32_t sc[MINE];
 };
 
+// What a block does.  Each role works it out for itself after it has its
+// registers: values that live across setmaxnreg are held to the smaller count
+// and spilled (measured: the softmax twice as slow).
+template <int KVB>
+struct KpUnit {
+    Kv4Seq q;
+    int seq, kh, rt, rows, cut, ncut;  // rows from this block's first to the sequence's last
+    int nblk, pos0;                    // blocks of positions of this piece, its first position
+    int nb[2], first_p[2], last_p[2];  // per tile: blocks it needs, position of its first and last row
+    __device__ __forceinline__ bool load(const Kv4AttnArgs &a, int row_tiles, int cuts) {
+        // later rows first, they see the most; pieces of a unit side by side
+        int u = blockIdx.x;
+        cut = u % cuts;
+        u /= cuts;
+        kh = u % a.c.n_kv;
+        u /= a.c.n_kv;
+        seq = u % a.c.n_seqs;
+        rt = row_tiles - 1 - u / a.c.n_seqs;
+        q.load(a, seq);
+        rows = q.nq * a.gq - rt * KP_ROWS;
+        if (rows <= 0) return false;
+        const int start = a.window > 0 ? max(0, q.before + rt * KP_ROWS / a.gq - a.window + 1) & ~31 : 0;
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            const int r0 = rt * KP_ROWS + 128 * i, r1 = min(r0 + 127, q.nq * a.gq - 1);
+            first_p[i] = q.before + r0 / a.gq;
+            last_p[i] = q.before + r1 / a.gq;
+            nb[i] = 128 * i < rows ? max(0, (last_p[i] + 1 - start + KVB - 1) / KVB) : 0;
+        }
+        const int all = max(nb[0], nb[1]);
+        ncut = max(1, min(cuts, all));
+        if (cut >= ncut) return false;
+        const int b0 = (int)((long long)all * cut / ncut), b1 = (int)((long long)all * (cut + 1) / ncut);
+        nblk = b1 - b0;
+        pos0 = start + b0 * KVB;
+#pragma unroll
+        for (int i = 0; i < 2; i++) nb[i] = max(0, min(nb[i], b1) - b0);
+        return true;
+    }
+};
+
 template <int HD, bool SPLIT, typename T>
 __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, int row_tiles, int cuts) {
     using C = KpCfg<HD, SPLIT>;
@@ -117,40 +206,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     __shared__ uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full;
     __shared__ uint32_t tmem_base;
     __shared__ int s_last;
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
-    // ---- the unit: later rows first, they see the most; pieces of a unit side by side
-    int u = blockIdx.x;
-    const int cut = u % cuts;
-    u /= cuts;
-    const int kh = u % a.c.n_kv;
-    u /= a.c.n_kv;
-    const int seq = u % a.c.n_seqs, rt = row_tiles - 1 - u / a.c.n_seqs;
-    Kv4Seq q;
-    q.load(a, seq);
-    const int rows = q.nq * a.gq - rt * KP_ROWS;  // rows from this block's first to the sequence's last
-    if (rows <= 0) return;
-    const int before = q.before;                  // position of query 0
-    // tile i's last row's position, and the blocks of positions it needs from start on
-    const int j_first = rt * KP_ROWS / a.gq;
-    const int start = a.window > 0 ? max(0, before + j_first - a.window + 1) & ~31 : 0;
-    int nb[2], first_p[2], last_p[2];
-#pragma unroll
-    for (int i = 0; i < 2; i++) {
-        const int r0 = rt * KP_ROWS + 128 * i, r1 = min(r0 + 127, q.nq * a.gq - 1);
-        first_p[i] = before + r0 / a.gq;
-        last_p[i] = before + r1 / a.gq;
-        nb[i] = 128 * i < rows ? max(0, (last_p[i] + 1 - start + KVB - 1) / KVB) : 0;
+    {
+        KpUnit<KVB> u;
+        if (!u.load(a, row_tiles, cuts)) return;  // the whole block
     }
-    const int all_blocks = max(nb[0], nb[1]);
-    const int ncut = max(1, min(cuts, all_blocks));
-    if (cut >= ncut) return;
-    const int blk0 = (int)((long long)all_blocks * cut / ncut), blk1 = (int)((long long)all_blocks * (cut + 1) / ncut);
-    const int nblk = blk1 - blk0;
-#pragma unroll
-    for (int i = 0; i < 2; i++) nb[i] = max(0, min(nb[i], blk1) - blk0);
-    const int pos0 = start + blk0 * KVB;  // of this piece
-
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
             mbar_init(&k_full[i], KP_DEQ);
@@ -168,62 +229,73 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = tmem_base;
-    bool ok = true;
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REG_OTHER));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REG_OTHER) : "memory");
+        const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(&tmem_base), 0);
+        KpUnit<KVB> u;
+        u.load(a, row_tiles, cuts);
+        const Kv4Seq &q = u.q;
+        const int nblk = u.nblk, pos0 = u.pos0, seq = u.seq, kh = u.kh;
+        bool ok = true;
         if (warp == 15) {
             // ------------------------------------------------ MMA issuer
-            if (lane == 0 && nblk > 0) {
+            if (nblk > 0) {
                 constexpr uint32_t id_s = umma_idesc_f16(128, KVB);
                 constexpr uint32_t id_o = umma_idesc_f16(128, HD) | (1u << 16);  // B with its N contiguous
+                // descriptors of the tiles' starts; an offset adds its sixteenth
+                const uint64_t q_desc = umma_desc_sw128(smem_u32(sq)), k_desc = umma_desc_sw128(smem_u32(sk));
+                const uint64_t v_desc = desc_v(smem_u32(sv), KVB * 128);
                 auto scores = [&](int i, int b) {
-                    const uint32_t qa = smem_u32(sq + i * C::Q_TILE), kb = smem_u32(sk + (b & 1) * C::KV_STAGE);
+                    const uint64_t qd = q_desc + (uint32_t)(i * C::Q_TILE / 16), kd = k_desc + (uint32_t)((b & 1) * C::KV_STAGE / 16);
+                    const uint32_t d = tmem + i * C::TM_S;
 #pragma unroll
                     for (int k = 0; k < HD / 16; k++) {
-                        const uint32_t ko = (k >> 2) * (KVB * 128) + (k & 3) * 32, qo = (k >> 2) * (128 * 128) + (k & 3) * 32;
-                        tc_mma_f16(tmem + i * C::TM_S, umma_desc_sw128(qa + qo), umma_desc_sw128(kb + ko), id_s, k > 0);
-                        if (SPLIT)
-                            tc_mma_f16(tmem + i * C::TM_S, umma_desc_sw128(qa + C::Q_HALF + qo), umma_desc_sw128(kb + ko), id_s, 1u);
+                        const int ko = (k >> 2) * (KVB * 128) + (k & 3) * 32, qo = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                        mma_ss(d, qd + qo / 16, kd + ko / 16, id_s, k > 0);
+                        if (SPLIT) mma_ss(d, qd + (C::Q_HALF + qo) / 16, kd + ko / 16, id_s, 1u);
                     }
-                    tc_commit(&s_full[i]);
+                    mma_commit(&s_full[i]);
                 };
                 auto products = [&](int i, int b) {
-                    const uint32_t vb = smem_u32(sv + (b & 1) * C::KV_STAGE), o = tmem + 2 * C::TM_S + i * C::TM_O;
+                    const uint64_t vd = v_desc + (uint32_t)((b & 1) * C::KV_STAGE / 16);
+                    const uint32_t o = tmem + 2 * C::TM_S + i * C::TM_O, p = tmem + i * C::TM_S;
 #pragma unroll
                     for (int k = 0; k < KVB / 16; k++) {
-                        // weights of 32 positions: 16 columns of hi, then 16 of lo
-                        const uint32_t p = tmem + i * C::TM_S + (k >> 1) * 32 + (k & 1) * 8;
-                        const uint64_t d = desc_v(vb + k * 2048, KVB * 128);
-                        tc_mma_f16_ts(o, p, d, id_o, k > 0);
-                        if (SPLIT) tc_mma_f16_ts(o, p + 16, d, id_o, 1u);
+                        // weights of CH positions: CH / 2 columns of hi, then of lo
+                        const int at = k * 16 / C::CH * C::CH + k * 16 % C::CH / 2;
+                        mma_ts(o, p + at, vd + k * 2048 / 16, id_o, k > 0);
+                        if (SPLIT) mma_ts(o, p + at + C::CH / 2, vd + k * 2048 / 16, id_o, 1u);
                     }
                 };
-                ok = mbar_wait(&q_full, 0) && mbar_wait(&k_full[0], 0);
+                ok = kp_wait(&q_full, 0) && kp_wait(&k_full[0], 0);
                 tc_fence_after();
                 if (ok) {
+#pragma unroll
                     for (int i = 0; i < 2; i++)
-                        if (nb[i] > 0) scores(i, 0);
-                    tc_commit(&k_empty[0]);
+                        if (u.nb[i] > 0) scores(i, 0);
+                    mma_commit(&k_empty[0]);
                 }
                 for (int b = 0; b < nblk && ok; b++) {
-                    const uint32_t par = (b >> 1) & 1, par1 = ((b + 1) >> 1) & 1;
-                    ok = mbar_wait(&v_full[b & 1], par);
-                    if (ok && b + 1 < nblk) ok = mbar_wait(&k_full[(b + 1) & 1], par1);
-                    for (int i = 0; i < 2 && ok; i++) {
-                        if (b >= nb[i]) continue;
-                        ok = mbar_wait(&p_full[i], b & 1);
-                        if (!ok) break;
+                    ok = kp_wait(&v_full[b & 1], (b >> 1) & 1);
+#pragma unroll
+                    for (int i = 0; i < 2; i++) {
+                        if (b >= u.nb[i] || !ok) continue;
+                        ok = kp_wait(&p_full[i], b & 1);
+                        if (!ok) continue;
                         tc_fence_after();
                         products(i, b);
-                        if (b + 1 < nb[i]) scores(i, b + 1);
-                        else tc_commit(&o_full[i]);
+                        if (b + 1 < u.nb[i]) {
+                            ok = kp_wait(&k_full[(b + 1) & 1], ((b + 1) >> 1) & 1);
+                            if (ok) scores(i, b + 1);
+                        } else {
+                            mma_commit(&o_full[i]);
+                        }
                     }
-                    tc_commit(&v_empty[b & 1]);
-                    if (b + 1 < nblk) tc_commit(&k_empty[(b + 1) & 1]);
+                    mma_commit(&v_empty[b & 1]);
+                    if (b + 1 < nblk) mma_commit(&k_empty[(b + 1) & 1]);
                 }
-                if (!ok) atomicExch(a.err, KP_ERR);
+                if (!ok && lane == 0) atomicExch(a.err, KP_ERR);
             }
         } else {
             // ------------------------------------------------ codes -> f16
@@ -259,7 +331,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
             load(vp, 0, false);
             for (int b = 0; b < nblk && ok; b++) {
                 const int st = b & 1;
-                if (b >= 2) ok = mbar_wait(&k_empty[st], ((b >> 1) - 1) & 1);
+                if (b >= 2) ok = kp_wait(&k_empty[st], ((b >> 1) - 1) & 1);
                 if (!ok) break;
                 uint8_t *ks = sk + st * C::KV_STAGE, *vs = sv + st * C::KV_STAGE;
 #pragma unroll
@@ -295,7 +367,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                 if (lane == 0) mbar_arrive(&k_full[st]);
                 load(kp, b + 1, true);
 
-                if (b >= 2) ok = mbar_wait(&v_empty[st], ((b >> 1) - 1) & 1);
+                if (b >= 2) ok = kp_wait(&v_empty[st], ((b >> 1) - 1) & 1);
                 if (!ok) break;
                 const int bp = pos0 + b * KVB;
 #pragma unroll
@@ -338,9 +410,17 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
             if (!ok && lane == 0) atomicExch(a.err, KP_ERR);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_REG_SOFTMAX));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_REG_SOFTMAX) : "memory");
+        const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(&tmem_base), 0);
+        KpUnit<KVB> u;
+        u.load(a, row_tiles, cuts);
+        const Kv4Seq &q = u.q;
+        const int rt = u.rt, kh = u.kh, seq = u.seq, rows = u.rows, cut = u.cut, ncut = u.ncut, pos0 = u.pos0, before = q.before;
+        bool ok = true;
         // ---------------------------------------------------- softmax, thread = row
-        const int i = warp >> 2, r = tid & 127, row = rt * KP_ROWS + 128 * i + r;
+        const int i = warp >> 2, blocks = i ? u.nb[1] : u.nb[0];
+        const int first_row_p = i ? u.first_p[1] : u.first_p[0], last_row_p = i ? u.last_p[1] : u.last_p[0];
+        const int r = tid & 127, row = rt * KP_ROWS + 128 * i + r;
         const int j = row / a.gq, h = kh * a.gq + row - j * a.gq;
         const bool live = j < q.nq;
         const int hi = live ? before + j : -1, lo = a.window > 0 ? hi - a.window + 1 : 0;
@@ -388,68 +468,95 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
         float o[HD];
 #pragma unroll
         for (int k = 0; k < HD; k++) o[k] = 0.f;
-        auto add_products = [&]() {  // the last block's, with the factor that its maximum gave
-#pragma unroll
-            for (int c = 0; c < HD / 32; c++) {
-                float v[32];
-                tmem_ld32(to + 32 * c, v);
-#pragma unroll
-                for (int k = 0; k < 32; k++) o[32 * c + k] = fmaf(o[32 * c + k], alpha, v[k]);
+        constexpr int CH = C::CH, NC = KVB / CH;
+        uint32_t ra[CH], rb[CH];
+        // a block's columns of this lane, `f` called with each CH of them while the next ones load.  Blocks that every
+        // row sees whole take straight-line code: a branch costs some 50 cycles here (the roles' code is far apart)
+        auto columns = [&](auto edge, auto &&f) {
+            constexpr int U = decltype(edge)::value ? 1 : NC / 2;
+            tmem_ld_start(ts, ra);
+#pragma unroll U
+            for (int c = 0; c < NC; c += 2) {
+                tmem_ld_wait(ra);
+                tmem_ld_start(ts + CH * (c + 1), rb);
+                f(c, ra);
+                tmem_ld_wait(rb);
+                if (c + 2 < NC) tmem_ld_start(ts + CH * (c + 2), ra);
+                f(c + 1, rb);
             }
         };
-        for (int b = 0; b < nb[i]; b++) {
-            ok = mbar_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
+        auto add_products = [&]() {  // the last block's, with the factor that its maximum gave
+            tmem_ld_start(to, ra);
+#pragma unroll
+            for (int c = 0; c < HD / CH; c += 2) {
+                tmem_ld_wait(ra);
+                tmem_ld_start(to + CH * (c + 1), rb);
+#pragma unroll
+                for (int k = 0; k < CH; k++) o[CH * c + k] = fmaf(o[CH * c + k], alpha, __uint_as_float(ra[k]));
+                tmem_ld_wait(rb);
+                if (c + 2 < HD / CH) tmem_ld_start(to + CH * (c + 2), ra);
+#pragma unroll
+                for (int k = 0; k < CH; k++) o[CH * (c + 1) + k] = fmaf(o[CH * (c + 1) + k], alpha, __uint_as_float(rb[k]));
+            }
+        };
+        for (int b = 0; b < blocks; b++) {
+            ok = kp_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
             if (!ok) break;
             tc_fence_after();
             if (b > 0) add_products();
             const int bp = pos0 + b * KVB;
-            const bool edge = bp + KVB - 1 > first_p[i] || (a.window > 0 && bp < last_p[i] - a.window + 1);
-            const int c_lo = max(lo - bp, 0);
-            const unsigned span = (unsigned)max(hi - bp - c_lo, -1) + 1u;  // columns c_lo .. c_lo + span - 1 are seen
-            float top = -INFINITY;
-#pragma unroll
-            for (int c = 0; c < KVB / 32; c++) {
-                float v[32];
-                tmem_ld32(ts + 32 * c, v);
-                if (edge) {
-#pragma unroll
-                    for (int k = 0; k < 32; k++) v[k] = (unsigned)(32 * c + k - c_lo) < span ? v[k] : -INFINITY;
-                }
-#pragma unroll
-                for (int k = 0; k < 32; k += 2) top = max3(top, v[k], v[k + 1]);
-            }
-            const float mn = top == -INFINITY ? m : fmaxf(m, top * factor), mm = mn == -INFINITY ? 0.f : mn;
-            alpha = kp_ex2(m - mm);
-            m = mn;
             float s0 = 0.f, s1 = 0.f;
+            auto block = [&](auto edge) {
+                constexpr bool EDGE = decltype(edge)::value;
+                float top = -INFINITY;
+                columns(edge, [&](int c, uint32_t (&r)[CH]) {
+                    if (EDGE) {
+                        const int up = hi - bp - CH * c, down = lo - bp - CH * c;
 #pragma unroll
-            for (int c = 0; c < KVB / 32; c++) {
-                float v[32];
-                tmem_ld32(ts + 32 * c, v);
-                uint32_t w[32];
-#pragma unroll
-                for (int k = 0; k < 32; k += 2) {
-                    float e0 = kp_ex2(fmaf(v[k], factor, -mm)), e1 = kp_ex2(fmaf(v[k + 1], factor, -mm));
-                    if (edge) {
-                        e0 = (unsigned)(32 * c + k - c_lo) < span ? e0 : 0.f;
-                        e1 = (unsigned)(32 * c + k + 1 - c_lo) < span ? e1 : 0.f;
+                        for (int k = 0; k < CH; k++) r[k] = k <= up && k >= down ? r[k] : 0xff800000u;
                     }
-                    s0 += e0;
-                    s1 += e1;
-                    if (SPLIT) kp_split(e0, e1, w[k / 2], w[16 + k / 2]);
-                    else w[k / 2] = kp_h2(e0, e1);
-                }
-                if (SPLIT) tmem_st32(ts + 32 * c, w);
-                else tmem_st16(ts + 32 * c, w);
-            }
+                    float t4[4];
+#pragma unroll
+                    for (int k = 0; k < 4; k++)
+                        t4[k] = max3(__uint_as_float(r[k]), __uint_as_float(r[k + 4]), __uint_as_float(r[k + 8]));
+#pragma unroll
+                    for (int k = 0; k < 4; k += 2) t4[k] = max3(t4[k], __uint_as_float(r[12 + k]), __uint_as_float(r[13 + k]));
+                    top = max3(top, max3(t4[0], t4[1], t4[2]), t4[3]);
+                });
+                const float mn = top == -INFINITY ? m : fmaxf(m, top * factor), mm = mn == -INFINITY ? 0.f : mn;
+                alpha = kp_ex2(m - mm);
+                m = mn;
+                columns(edge, [&](int c, uint32_t (&r)[CH]) {
+                    uint32_t w[SPLIT ? CH : CH / 2];
+                    float e[CH];
+#pragma unroll
+                    for (int k = 0; k < CH; k++) e[k] = kp_ex2(fmaf(__uint_as_float(r[k]), factor, -mm));
+                    if (EDGE) {
+                        const int up = hi - bp - CH * c, down = lo - bp - CH * c;
+#pragma unroll
+                        for (int k = 0; k < CH; k++) e[k] = k <= up && k >= down ? e[k] : 0.f;
+                    }
+#pragma unroll
+                    for (int k = 0; k < CH; k += 2) {
+                        s0 += e[k];
+                        s1 += e[k + 1];
+                        if constexpr (SPLIT) kp_split(e[k], e[k + 1], w[k / 2], w[CH / 2 + k / 2]);
+                        else w[k / 2] = kp_h2(e[k], e[k + 1]);
+                    }
+                    tmem_st(ts + CH * c, w);
+                });
+            };
+            // some row does not see some position of the block
+            if (bp + KVB - 1 > first_row_p || (a.window > 0 && bp <= last_row_p - a.window)) block(std::true_type{});
+            else block(std::false_type{});
             l = fmaf(l, alpha, s0 + s1);
             tmem_wait_st();
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&p_full[i]);
         }
-        if (nb[i] > 0 && ok) {
-            ok = mbar_wait(&o_full[i], 0);
+        if (blocks > 0 && ok) {
+            ok = kp_wait(&o_full[i], 0);
             tc_fence_after();
             if (ok) add_products();
         }
@@ -515,7 +622,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     __syncthreads();
     if (warp == 15) {
         tc_fence_after();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem_base, 512);
     }
 }
 
