@@ -31,8 +31,6 @@ constexpr int KP_ROWS = 256;        // rows of a block
 constexpr int KP_THREADS = 512;
 constexpr int KP_DEQ = 7;           // warps 8-14
 constexpr int KP_ERR = 42;
-constexpr int KP_REG_SOFTMAX = 192, KP_REG_OTHER = 64;
-static_assert(KP_REG_SOFTMAX + KP_REG_OTHER == 256, "two warpgroups of each out of 512 x 128 registers");
 
 template <int HD, bool SPLIT>
 struct KpCfg {
@@ -43,12 +41,28 @@ struct KpCfg {
     static constexpr int KV_STAGE = PLANES * KVB * 128;        // bytes of a K (or V) stage
     static constexpr int SMEM = 2 * Q_TILE + 4 * KV_STAGE + 1024;
     static constexpr int TM_S = KVB, TM_O = HD;                // TMEM columns of a tile
-    static constexpr int CH = 16;                              // score columns a thread has at a time (two of them)
+    static constexpr int CH = SPLIT ? 16 : 32;                 // positions whose weights lie together in TMEM
+    // registers of the softmax warps, of the others: two warpgroups of each out of 512 x 128
+    static constexpr int REG_SOFTMAX = SPLIT ? 192 : 176, REG_OTHER = 256 - REG_SOFTMAX;
 };
 
 __device__ __forceinline__ float kp_ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// two fp32 operations in one instruction
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 x, x, y, z;\n mov.b64 {%0, %1}, x;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 x, x, y;\n mov.b64 {%0, %1}, x;\n}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -135,9 +149,9 @@ __device__ __forceinline__ uint32_t kp_h2(float a, float b) {
 }
 __device__ __forceinline__ void kp_split(float a, float b, uint32_t &hi, uint32_t &lo) {
     const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
+    const float2 f = __half22float2(h), r = fma2(f, make_float2(-1.f, -1.f), make_float2(a, b));
     hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = kp_h2(a - f.x, b - f.y);
+    lo = kp_h2(r.x, r.y);
 }
 __device__ __forceinline__ uint32_t kp_scale(uint32_t w, int b) { return __byte_perm(w, 0u, (b << 12) | (b << 4) | 0x404); }
 __device__ __forceinline__ uint4 kp_eight(uint32_t codes, uint32_t f) {  // eight codes -> f16
@@ -206,6 +220,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     __shared__ uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full;
     __shared__ uint32_t tmem_base;
     __shared__ int s_last;
+    __shared__ float s_factor[KP_ROWS];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
     {
@@ -231,7 +246,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     tc_fence_after();
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(KP_REG_OTHER) : "memory");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_OTHER) : "memory");
         const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(&tmem_base), 0);
         KpUnit<KVB> u;
         u.load(a, row_tiles, cuts);
@@ -264,7 +279,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                     for (int k = 0; k < KVB / 16; k++) {
                         // weights of CH positions: CH / 2 columns of hi, then of lo
                         const int at = k * 16 / C::CH * C::CH + k * 16 % C::CH / 2;
-                        mma_ts(o, p + at, vd + k * 2048 / 16, id_o, k > 0);
+                        mma_ts(o, p + at, vd + k * 2048 / 16, id_o, k > 0 || (!SPLIT && b > 0));
                         if (SPLIT) mma_ts(o, p + at + C::CH / 2, vd + k * 2048 / 16, id_o, 1u);
                     }
                 };
@@ -410,7 +425,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
             if (!ok && lane == 0) atomicExch(a.err, KP_ERR);
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(KP_REG_SOFTMAX) : "memory");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFTMAX) : "memory");
         const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(&tmem_base), 0);
         KpUnit<KVB> u;
         u.load(a, row_tiles, cuts);
@@ -424,141 +439,239 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
         const int j = row / a.gq, h = kh * a.gq + row - j * a.gq;
         const bool live = j < q.nq;
         const int hi = live ? before + j : -1, lo = a.window > 0 ? hi - a.window + 1 : 0;
-        float factor;
-        {   // the row's queries, scaled to below 2 by a power of two, into the swizzled tile; the scale's sign goes with them
-            const T *src = static_cast<const T *>(a.q) + (int64_t)(q.q0 + j) * a.ldq + (int64_t)h * HD;
-            float top = 0.f;
-#pragma unroll 1
-            for (int c = 0; c < HD; c += 16) {
-                float x[16];
-                if (live) load_row<16>(src + c, a.q_wide, x);
+        {   // the queries, scaled to below 2 by a power of two per row, into the swizzled tile; the scale's sign goes with
+            // them.  A row takes HD / 8 lanes, a lane one 16-byte chunk of the tile.
+            constexpr int L = HD / 8, STEP = 32 / L, N = 32 / STEP;
+            const int first = 32 * (warp & 3), c = lane % L;
+            float x[N][8];
 #pragma unroll
-                for (int k = 0; k < 16; k++) top = live ? fmaxf(top, fabsf(x[k])) : 0.f;
-            }
-            const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-            const float down = __uint_as_float((254u - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
-            factor = fabsf(a.scale) * LOG2E * __uint_as_float(e << 23);
-            uint8_t *dst = sq + i * C::Q_TILE + r * 128;
-#pragma unroll 1
-            for (int c = 0; c < HD / 16; c++) {
-                float x[16];
-                if (live) load_row<16>(src + c * 16, a.q_wide, x);
+            for (int k = 0; k < N; k++) {
+                const int rr = rt * KP_ROWS + 128 * i + first + k * STEP + lane / L, jj = rr / a.gq;
+                if (jj < q.nq) {
+                    load_row<8>(static_cast<const T *>(a.q) + (int64_t)(q.q0 + jj) * a.ldq +
+                                    (int64_t)(kh * a.gq + rr - jj * a.gq) * HD + 8 * c, a.q_wide, x[k]);
+                } else {
 #pragma unroll
-                for (int half = 0; half < 2; half++) {
-                    uint32_t vh[4], vl[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const float x0 = live ? x[8 * half + 2 * k] * down : 0.f, x1 = live ? x[8 * half + 2 * k + 1] * down : 0.f;
-                        if (SPLIT) kp_split(x0, x1, vh[k], vl[k]);
-                        else vh[k] = kp_h2(x0, x1);
-                    }
-                    const int chunk = 2 * c + half;
-                    uint8_t *at = dst + (chunk >> 3) * (128 * 128) + (((chunk & 7) ^ (r & 7)) << 4);
-                    *reinterpret_cast<uint4 *>(at) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
-                    if (SPLIT) *reinterpret_cast<uint4 *>(at + C::Q_HALF) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
+                    for (int e = 0; e < 8; e++) x[k][e] = 0.f;
                 }
+                if (SPLIT && HD == 128 && k % 8 == 7) asm volatile("" ::: "memory");  // eight rows' loads at a time
+            }
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                float top = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[k][e]));
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+                const float down = __uint_as_float((254u - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
+                uint32_t vh[4], vl[4];
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    if (SPLIT) kp_split(x[k][2 * y] * down, x[k][2 * y + 1] * down, vh[y], vl[y]);
+                    else vh[y] = kp_h2(x[k][2 * y] * down, x[k][2 * y + 1] * down);
+                }
+                const int rr = first + k * STEP + lane / L;
+                uint8_t *at = sq + i * C::Q_TILE + rr * 128 + (c >> 3) * (128 * 128) + (((c & 7) ^ (rr & 7)) << 4);
+                *reinterpret_cast<uint4 *>(at) = make_uint4(vh[0], vh[1], vh[2], vh[3]);
+                if (SPLIT) *reinterpret_cast<uint4 *>(at + C::Q_HALF) = make_uint4(vl[0], vl[1], vl[2], vl[3]);
+                if (c == 0) s_factor[128 * i + rr] = fabsf(a.scale) * LOG2E * __uint_as_float(e << 23);
             }
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full);
         }
+        const float factor = fmaxf(s_factor[128 * i + r], 1e-37f);  // above zero: a masked -infinity times it stays one
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + lanes + i * C::TM_S, to = tmem + lanes + 2 * C::TM_S + i * C::TM_O;
-        float m = -INFINITY, l = 0.f, alpha = 1.f;
+        float m = -INFINITY, l = 0.f;
         float o[HD];
+        if constexpr (SPLIT) {
+            // f32: O in registers, each block's product added with the factor that its maximum gave
+            float alpha = 1.f;
 #pragma unroll
-        for (int k = 0; k < HD; k++) o[k] = 0.f;
-        constexpr int CH = C::CH, NC = KVB / CH;
-        uint32_t ra[CH], rb[CH];
-        // a block's columns of this lane, `f` called with each CH of them while the next ones load.  Blocks that every
-        // row sees whole take straight-line code: a branch costs some 50 cycles here (the roles' code is far apart)
-        auto columns = [&](auto edge, auto &&f) {
-            constexpr int U = decltype(edge)::value ? 1 : NC / 2;
-            tmem_ld_start(ts, ra);
+            for (int k = 0; k < HD; k++) o[k] = 0.f;
+            constexpr int CH = C::CH, NC = KVB / CH;
+            uint32_t ra[CH], rb[CH];
+            // a block's columns of this lane, `f` called with each CH of them while the next ones load.  Blocks that every
+            // row sees whole take straight-line code: a branch costs some 50 cycles here (the roles' code is far apart)
+            auto columns = [&](auto edge, auto &&f) {
+                constexpr int U = decltype(edge)::value ? 1 : NC / 2;
+                tmem_ld_start(ts, ra);
 #pragma unroll U
-            for (int c = 0; c < NC; c += 2) {
-                tmem_ld_wait(ra);
-                tmem_ld_start(ts + CH * (c + 1), rb);
-                f(c, ra);
-                tmem_ld_wait(rb);
-                if (c + 2 < NC) tmem_ld_start(ts + CH * (c + 2), ra);
-                f(c + 1, rb);
-            }
-        };
-        auto add_products = [&]() {  // the last block's, with the factor that its maximum gave
-            tmem_ld_start(to, ra);
-#pragma unroll
-            for (int c = 0; c < HD / CH; c += 2) {
-                tmem_ld_wait(ra);
-                tmem_ld_start(to + CH * (c + 1), rb);
-#pragma unroll
-                for (int k = 0; k < CH; k++) o[CH * c + k] = fmaf(o[CH * c + k], alpha, __uint_as_float(ra[k]));
-                tmem_ld_wait(rb);
-                if (c + 2 < HD / CH) tmem_ld_start(to + CH * (c + 2), ra);
-#pragma unroll
-                for (int k = 0; k < CH; k++) o[CH * (c + 1) + k] = fmaf(o[CH * (c + 1) + k], alpha, __uint_as_float(rb[k]));
-            }
-        };
-        for (int b = 0; b < blocks; b++) {
-            ok = kp_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
-            if (!ok) break;
-            tc_fence_after();
-            if (b > 0) add_products();
-            const int bp = pos0 + b * KVB;
-            float s0 = 0.f, s1 = 0.f;
-            auto block = [&](auto edge) {
-                constexpr bool EDGE = decltype(edge)::value;
-                float top = -INFINITY;
-                columns(edge, [&](int c, uint32_t (&r)[CH]) {
-                    if (EDGE) {
-                        const int up = hi - bp - CH * c, down = lo - bp - CH * c;
-#pragma unroll
-                        for (int k = 0; k < CH; k++) r[k] = k <= up && k >= down ? r[k] : 0xff800000u;
-                    }
-                    float t4[4];
-#pragma unroll
-                    for (int k = 0; k < 4; k++)
-                        t4[k] = max3(__uint_as_float(r[k]), __uint_as_float(r[k + 4]), __uint_as_float(r[k + 8]));
-#pragma unroll
-                    for (int k = 0; k < 4; k += 2) t4[k] = max3(t4[k], __uint_as_float(r[12 + k]), __uint_as_float(r[13 + k]));
-                    top = max3(top, max3(t4[0], t4[1], t4[2]), t4[3]);
-                });
-                const float mn = top == -INFINITY ? m : fmaxf(m, top * factor), mm = mn == -INFINITY ? 0.f : mn;
-                alpha = kp_ex2(m - mm);
-                m = mn;
-                columns(edge, [&](int c, uint32_t (&r)[CH]) {
-                    uint32_t w[SPLIT ? CH : CH / 2];
-                    float e[CH];
-#pragma unroll
-                    for (int k = 0; k < CH; k++) e[k] = kp_ex2(fmaf(__uint_as_float(r[k]), factor, -mm));
-                    if (EDGE) {
-                        const int up = hi - bp - CH * c, down = lo - bp - CH * c;
-#pragma unroll
-                        for (int k = 0; k < CH; k++) e[k] = k <= up && k >= down ? e[k] : 0.f;
-                    }
-#pragma unroll
-                    for (int k = 0; k < CH; k += 2) {
-                        s0 += e[k];
-                        s1 += e[k + 1];
-                        if constexpr (SPLIT) kp_split(e[k], e[k + 1], w[k / 2], w[CH / 2 + k / 2]);
-                        else w[k / 2] = kp_h2(e[k], e[k + 1]);
-                    }
-                    tmem_st(ts + CH * c, w);
-                });
+                for (int c = 0; c < NC; c += 2) {
+                    tmem_ld_wait(ra);
+                    tmem_ld_start(ts + CH * (c + 1), rb);
+                    f(c, ra);
+                    tmem_ld_wait(rb);
+                    if (c + 2 < NC) tmem_ld_start(ts + CH * (c + 2), ra);
+                    f(c + 1, rb);
+                }
             };
-            // some row does not see some position of the block
-            if (bp + KVB - 1 > first_row_p || (a.window > 0 && bp <= last_row_p - a.window)) block(std::true_type{});
-            else block(std::false_type{});
-            l = fmaf(l, alpha, s0 + s1);
-            tmem_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[i]);
-        }
-        if (blocks > 0 && ok) {
-            ok = kp_wait(&o_full[i], 0);
-            tc_fence_after();
-            if (ok) add_products();
+            auto add_products = [&]() {  // the last block's, with the factor that its maximum gave
+                auto add = [&](int k, uint32_t x, uint32_t y) {
+                    const float2 v = fma2(make_float2(o[k], o[k + 1]), make_float2(alpha, alpha),
+                                          make_float2(__uint_as_float(x), __uint_as_float(y)));
+                    o[k] = v.x;
+                    o[k + 1] = v.y;
+                };
+                tmem_ld_start(to, ra);
+#pragma unroll
+                for (int c = 0; c < HD / CH; c += 2) {
+                    tmem_ld_wait(ra);
+                    tmem_ld_start(to + CH * (c + 1), rb);
+#pragma unroll
+                    for (int k = 0; k < CH; k += 2) add(CH * c + k, ra[k], ra[k + 1]);
+                    tmem_ld_wait(rb);
+                    if (c + 2 < HD / CH) tmem_ld_start(to + CH * (c + 2), ra);
+#pragma unroll
+                    for (int k = 0; k < CH; k += 2) add(CH * (c + 1) + k, rb[k], rb[k + 1]);
+                }
+            };
+            for (int b = 0; b < blocks; b++) {
+                ok = kp_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
+                if (!ok) break;
+                tc_fence_after();
+                if (b > 0) add_products();
+                const int bp = pos0 + b * KVB;
+                float2 sum = make_float2(0.f, 0.f);
+                auto block = [&](auto edge) {
+                    constexpr bool EDGE = decltype(edge)::value;
+                    float top = -INFINITY;
+                    columns(edge, [&](int c, uint32_t (&r)[CH]) {
+                        if (EDGE) {
+                            const int up = hi - bp - CH * c, down = lo - bp - CH * c;
+#pragma unroll
+                            for (int k = 0; k < CH; k++) r[k] = k <= up && k >= down ? r[k] : 0xff800000u;
+                        }
+                        float t4[4];
+#pragma unroll
+                        for (int k = 0; k < 4; k++)
+                            t4[k] = max3(__uint_as_float(r[k]), __uint_as_float(r[k + 4]), __uint_as_float(r[k + 8]));
+#pragma unroll
+                        for (int k = 0; k < 4; k += 2) t4[k] = max3(t4[k], __uint_as_float(r[12 + k]), __uint_as_float(r[13 + k]));
+                        top = max3(top, max3(t4[0], t4[1], t4[2]), t4[3]);
+                    });
+                    const float mn = top == -INFINITY ? m : fmaxf(m, top * factor), mm = mn == -INFINITY ? 0.f : mn;
+                    alpha = kp_ex2(m - mm);
+                    m = mn;
+                    columns(edge, [&](int c, uint32_t (&r)[CH]) {
+                        uint32_t w[CH];
+                        float e[CH];
+#pragma unroll
+                        for (int k = 0; k < CH; k += 2) {
+                            const float2 x = fma2(make_float2(__uint_as_float(r[k]), __uint_as_float(r[k + 1])),
+                                                  make_float2(factor, factor), make_float2(-mm, -mm));
+                            e[k] = kp_ex2(x.x);
+                            e[k + 1] = kp_ex2(x.y);
+                        }
+                        if (EDGE) {
+                            const int up = hi - bp - CH * c, down = lo - bp - CH * c;
+#pragma unroll
+                            for (int k = 0; k < CH; k++) e[k] = k <= up && k >= down ? e[k] : 0.f;
+                        }
+#pragma unroll
+                        for (int k = 0; k < CH; k += 2) {
+                            sum = add2(sum, make_float2(e[k], e[k + 1]));
+                            kp_split(e[k], e[k + 1], w[k / 2], w[CH / 2 + k / 2]);
+                        }
+                        tmem_st(ts + CH * c, w);
+                    });
+                };
+                // some row does not see some position of the block
+                if (bp + KVB - 1 > first_row_p || (a.window > 0 && bp <= last_row_p - a.window)) block(std::true_type{});
+                else block(std::false_type{});
+                l = fmaf(l, alpha, sum.x + sum.y);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[i]);
+            }
+            if (blocks > 0 && ok) {
+                ok = kp_wait(&o_full[i], 0);
+                tc_fence_after();
+                if (ok) add_products();
+            }
+        } else {
+            // f16, bf16: O stays in TMEM; m is followed up, and O and l rescaled, only when a maximum exceeds it by 2^8
+            // (weights up to 256 keep their 11 bits in f16)
+            for (int b = 0; b < blocks; b++) {
+                ok = kp_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t r[KVB / 32][32];
+#pragma unroll
+                for (int c = 0; c < KVB / 32; c++) tmem_ld_start(ts + 32 * c, r[c]);
+#pragma unroll
+                for (int c = 0; c < KVB / 32; c++) tmem_ld_wait(r[c]);
+                const int bp = pos0 + b * KVB;
+                // some row does not see some position of the block
+                if (bp + KVB - 1 > first_row_p || (a.window > 0 && bp <= last_row_p - a.window)) {
+                    const int up = hi - bp, down = lo - bp;
+#pragma unroll
+                    for (int k = 0; k < KVB; k++) r[k / 32][k % 32] = k <= up && k >= down ? r[k / 32][k % 32] : 0xff800000u;
+                }
+                float t4[4];
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    t4[c] = -INFINITY;
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) t4[c] = max3(t4[c], __uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1]));
+                }
+                const float top = max3(fmaxf(t4[0], t4[1]), t4[2], t4[3]), need = top == -INFINITY ? -INFINITY : top * factor;
+                if (__any_sync(0xffffffffu, need > m + 8.f)) {  // m = -infinity: any number
+                    const float mn = fmaxf(m, need), alpha = mn == -INFINITY ? 1.f : kp_ex2(m - mn);
+                    m = mn;
+                    l *= alpha;
+                    if (b > 0) {
+#pragma unroll 1
+                        for (int c = 0; c < HD; c += 16) {
+                            uint32_t v[16];
+                            tmem_ld_start(to + c, v);
+                            tmem_ld_wait(v);
+#pragma unroll
+                            for (int k = 0; k < 16; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
+                            tmem_st(to + c, v);
+                        }
+                    }
+                }
+                const float mm = m == -INFINITY ? 0.f : m;
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+#pragma unroll
+                for (int c = 0; c < KVB / 32; c++) {
+                    uint32_t w[16];
+#pragma unroll
+                    for (int k = 0; k < 32; k += 2) {
+                        const float2 x = fma2(make_float2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])),
+                                              make_float2(factor, factor), make_float2(-mm, -mm));
+                        const float2 e = make_float2(kp_ex2(x.x), kp_ex2(x.y));
+                        sum[k / 2 % 2] = add2(sum[k / 2 % 2], e);
+                        w[k / 2] = kp_h2(e.x, e.y);
+                    }
+                    tmem_st(ts + 32 * c, w);
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&p_full[i]);
+            }
+#pragma unroll
+            for (int k = 0; k < HD; k++) o[k] = 0.f;
+            if (blocks > 0 && ok) {
+                ok = kp_wait(&o_full[i], 0);
+                tc_fence_after();
+                if (ok) {
+#pragma unroll
+                    for (int c = 0; c < HD; c += 32) {
+                        uint32_t v[32];
+                        tmem_ld_start(to + c, v);
+                        tmem_ld_wait(v);
+#pragma unroll
+                        for (int k = 0; k < 32; k++) o[c + k] = __uint_as_float(v[k]);
+                    }
+                }
+            }
         }
         if (!ok && lane == 0) atomicExch(a.err, KP_ERR);
         // ---- the row's result, or this piece's part of it
