@@ -42,7 +42,8 @@ struct KpCfg {
     static constexpr int SMEM = 2 * Q_TILE + 4 * KV_STAGE + 1024;
     static constexpr int TM_S = KVB, TM_O = HD;                // TMEM columns of a tile
     static constexpr int CH = SPLIT ? 16 : 32;                 // positions whose weights lie together in TMEM
-    // registers of the softmax warps, of the others: two warpgroups of each out of 512 x 128
+    // registers of the softmax warps, of the others: two warpgroups of each out of 512 x 128; launch_many checks that the
+    // block starts with as many (a setmaxnreg.inc beyond them would wait forever)
     static constexpr int REG_SOFTMAX = SPLIT ? 192 : 176, REG_OTHER = 256 - REG_SOFTMAX;
 };
 
@@ -111,15 +112,14 @@ __device__ __forceinline__ void tmem_st(uint32_t taddr, const uint32_t (&v)[N]) 
     else if constexpr (N == 16) tmem_st16(taddr, v);
     else tmem_st32(taddr, v);
 }
-// mbar_wait whose polls sleep in the hardware for up to a microsecond each: the other roles need the issue slots
+// mbar_wait of a whole warp, whose polls may sleep in the hardware: the other roles need the issue slots.  The lanes are
+// together again on return, with one answer (tcgen05 instructions and elections need the whole warp).
 __device__ __forceinline__ bool kp_wait(uint64_t *bar, uint32_t parity) {
-    for (uint32_t i = 0; i < MBAR_POLLS; i++) {
-        uint32_t done;
+    uint32_t done = 0;
+    for (uint32_t i = 0; i < MBAR_POLLS && !done; i++)
         asm volatile("{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
                      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity), "r"(1000u) : "memory");
-        if (done) return true;
-    }
-    return false;
+    return __all_sync(0xffffffffu, done);
 }
 // MMAs and commits issued by one elected lane of a converged warp: descriptors stay in uniform registers (from one
 // divergent lane each MMA cost some 100 cycles of moves)
@@ -747,11 +747,19 @@ int kv4_many_cuts(int64_t units, int64_t blocks) {
 
 template <int HD, bool SPLIT, typename T>
 static int launch_many(const Kv4AttnArgs &a, int row_tiles, int cuts, cudaStream_t st) {
-    constexpr int smem = KpCfg<HD, SPLIT>::SMEM;
-    TRY(ensure_smem(k_kv4_attn_many<HD, SPLIT, T>, smem));
+    using C = KpCfg<HD, SPLIT>;
+    TRY(ensure_smem(k_kv4_attn_many<HD, SPLIT, T>, C::SMEM));
+    static int regs = 0;  // of a thread at launch
+    if (!regs) {
+        cudaFuncAttributes f{};
+        MG_CUDA(cudaFuncGetAttributes(&f, k_kv4_attn_many<HD, SPLIT, T>));
+        regs = f.numRegs;
+    }
+    MG_REQUIRE(regs * KP_THREADS >= 256 * (C::REG_SOFTMAX + C::REG_OTHER), MG_ERR_CUDA,
+               "kv4_attn: built with %d registers a thread, too few for its split", regs);
     const int64_t blocks = (int64_t)row_tiles * a.c.n_seqs * a.c.n_kv * cuts;
     MG_REQUIRE(blocks < (1LL << 31), MG_ERR_ARG, "kv4_attn: too many rows");
-    k_kv4_attn_many<HD, SPLIT, T><<<(unsigned)blocks, KP_THREADS, smem, st>>>(a, row_tiles, cuts);
+    k_kv4_attn_many<HD, SPLIT, T><<<(unsigned)blocks, KP_THREADS, C::SMEM, st>>>(a, row_tiles, cuts);
     MG_CHECK_LAUNCH();
     return MG_OK;
 }
