@@ -14,6 +14,8 @@
 // Bound: HBM (one read of the logits).
 #include <string.h>
 
+#include <type_traits>
+
 #include "mg_kv4.cuh"
 
 namespace mg {
@@ -48,8 +50,9 @@ struct LpSmem {
     float red[3][LP_THREADS / 32];
     float cv[LP_CAND];
     int32_t ci[LP_CAND];
+    uint16_t who[LP_THREADS];  // threads whose maximum reaches the bound
     float bound;
-    int n, last;
+    int n, nwho, last;
 };
 
 __device__ __forceinline__ float lp_ex2(float x) {
@@ -63,29 +66,56 @@ __device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }
 
 // sum and weighted sum against a maximum m, moved to the maximum M >= m
 __device__ __forceinline__ void lp_move(float &s, float &w, float m, float M) {
-    const float d = fmaxf(m - M, -1e30f), f = lp_ex2(d * LP_LOG2E);  // m = -infinity: s = w = 0
+    const float d = fmaxf(m - M, -1e30f), f = lp_ex2(d * LP_LOG2E);  // m = -infinity: s = w = 0, and f is 0
     w = f * (w + s * d);
     s *= f;
 }
 
+// A thread's sums are against a reference r that follows its maximum m only when that is LP_AHEAD above it (e^40 times the
+// entries stays far inside fp32): a running maximum moves in some lane of a warp nearly every time.
+constexpr float LP_AHEAD = 40.f;
 struct LpAcc {
-    float m = -INFINITY, s = 0.f, w = 0.f;
+    float m = -INFINITY, r = -INFINITY, s = 0.f, w = 0.f;
+    // entries one after another, -infinity (and NaN, made so) among them
     template <int N>
-    __device__ __forceinline__ void add(const float (&v)[N]) {
-        float top = v[0];
-#pragma unroll
-        for (int i = 1; i < N; i++) top = fmaxf(top, v[i]);
-        if (top > m) {
-            lp_move(s, w, m, top);
-            m = top;
-        }
-        const float mm = m == -INFINITY ? 0.f : m;
+    __device__ __forceinline__ void add_any(const float (&v)[N]) {
+        const float rr = r == -INFINITY ? 0.f : r;
 #pragma unroll
         for (int i = 0; i < N; i++) {
-            const float d = fmaxf(v[i] - mm, -1e30f), e = lp_ex2(d * LP_LOG2E);
+            const float d = fmaxf(v[i] - rr, -1e30f), e = lp_ex2(d * LP_LOG2E);
             s += e;
             w = fmaf(e, d, w);
         }
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&v)[N]) {
+        float top = m;
+#pragma unroll
+        for (int i = 0; i + 1 < N; i += 2) top = max3(top, v[i], v[i + 1]);
+        if (N & 1) top = fmaxf(top, v[N - 1]);
+        m = top;
+        if (top > r + LP_AHEAD) {  // r = -infinity: any number
+            lp_move(s, w, r, top);
+            r = top;
+        }
+        if constexpr (N % 2 == 0) {
+            float2 es = make_float2(0.f, 0.f), ws = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < N; i += 2) {
+                const float2 d = add2(make_float2(v[i], v[i + 1]), make_float2(-r, -r));
+                const float2 t = mul2(d, make_float2(LP_LOG2E, LP_LOG2E));
+                const float2 e = make_float2(lp_ex2(t.x), lp_ex2(t.y));
+                es = add2(es, e);
+                ws = fma2(e, d, ws);
+            }
+            const float wx = ws.x + ws.y;
+            if (wx == wx) {  // a -infinity or NaN entry (or nothing else yet) makes it NaN
+                s += es.x + es.y;
+                w += wx;
+                return;
+            }
+        }
+        add_any(v);
     }
 };
 
@@ -111,12 +141,39 @@ struct LpSpan {
     }
     __device__ __forceinline__ uint4 vec(int i) const { return __ldg(reinterpret_cast<const uint4 *>(x + va) + i); }
     static __device__ __forceinline__ void unpack(const uint4 &q, float *v) {
-        T e[E];
-        memcpy(e, &q, 16);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) {  // an operation an entry
+            const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int i = 0; i < E; i++) v[i] = to_f32(e[i]);
+            for (int i = 0; i < 4; i++) {
+                v[2 * i] = __uint_as_float(w[i] << 16);
+                v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        } else {
+            T e[E];
+            memcpy(e, &q, 16);
+#pragma unroll
+            for (int i = 0; i < E; i++) v[i] = to_f32(e[i]);
+        }
     }
 };
+
+// With fewer than `top` possible tokens in [a, b) (n of them, ranked already)
+// the next are the first banned ones (-infinity, NaN) by index: warp 0 looks
+// for them from a on, and all but n entries are such.
+template <typename T, typename F>
+__device__ __forceinline__ void lp_banned(const T *x, int64_t a, int64_t b, int n, int top, F &&out) {
+    if (threadIdx.x >= 32) return;
+    int r = n;
+    for (int64_t i0 = a; i0 < b && r < top; i0 += 32) {
+        const int64_t i = i0 + threadIdx.x;
+        const bool is = i < b && clean(to_f32(x[i])) == -INFINITY;
+        const unsigned who = __ballot_sync(0xffffffffu, is);
+        const int mine = r + __popc(who & ((1u << threadIdx.x) - 1u));
+        if (is && mine < top) out(mine, -INFINITY, (int32_t)i);
+        r += __popc(who);
+    }
+    for (r += threadIdx.x; r < top; r += 32) out(r, -INFINITY, -1);
+}
 
 // ranks the candidates sm.cv / sm.ci (n of them, distinct indexes) and calls out(rank, value, index) for the best `top`
 template <typename F>
@@ -128,7 +185,6 @@ __device__ __forceinline__ void lp_rank(const LpSmem &sm, int n, int top, F &&ou
         for (int j = 0; j < n; j++) r += better(sm.cv[j], sm.ci[j], v, id);
         if (r < top) out(r, v, id);
     }
-    for (int r = n + threadIdx.x; r < top; r += LP_THREADS) out(r, -INFINITY, -1);
 }
 
 // the best `top` of [a, b) one after another, a pass for each: where the candidates do not fit (rows of equal entries,
@@ -173,7 +229,7 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
     const T *x = static_cast<const T *>(a.x) + (int64_t)row * a.ldx;
     const int64_t p0 = a.V * part / a.splits, p1 = a.V * (part + 1) / a.splits;
     const LpSpan<T> sp(x, p0, p1);
-    if (tid == 0) sm.n = 0;
+    if (tid == 0) sm.n = sm.nwho = 0;
 
     // ---- the pass
     LpAcc acc;
@@ -189,10 +245,14 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
         uint4 q[LP_UNROLL];
 #pragma unroll
         for (int k = 0; k < LP_UNROLL; k++) q[k] = sp.vec(i + k * LP_THREADS);
-        float v[LP_UNROLL * E];
+        constexpr int AT = 16 / E;  // vectors of 16 entries
 #pragma unroll
-        for (int k = 0; k < LP_UNROLL; k++) LpSpan<T>::unpack(q[k], v + k * E);
-        acc.add(v);
+        for (int k = 0; k < LP_UNROLL; k += AT) {
+            float v[16];
+#pragma unroll
+            for (int j = 0; j < AT; j++) LpSpan<T>::unpack(q[k + j], v + j * E);
+            acc.add(v);
+        }
     }
     for (; i < sp.nv; i += LP_THREADS) {
         float v[E];
@@ -209,7 +269,7 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
     const float gm = sm.gmax[lane];
     const float M = warp_max(gm);
     float s = acc.s, w = acc.w;
-    lp_move(s, w, acc.m, M == -INFINITY ? 0.f : M);
+    lp_move(s, w, acc.r, M == -INFINITY ? 0.f : M);
     s = warp_sum(s);
     w = warp_sum(w);
     if (lane == 0) {
@@ -237,7 +297,7 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
     if (a.top > 0) {
         const float bound = sm.bound;
         auto take = [&](float v, int64_t at) {
-            if (v >= bound) {
+            if (v >= bound && v > -INFINITY) {
                 const int k = atomicAdd(&sm.n, 1);
                 if (k < LP_CAND) {
                     sm.cv[k] = v;
@@ -247,16 +307,18 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
         };
         const int64_t ei = sp.edge(tid);
         if (ei >= 0) take(clean(to_f32(x[ei])), ei);
-        unsigned who = __ballot_sync(0xffffffffu, acc.m >= bound);
-        while (who) {  // a warp reads one thread's vectors together
-            const int t = warp * 32 + __ffs(who) - 1;
-            who &= who - 1;
-            for (int k = t + lane * LP_THREADS; k < sp.nv; k += 32 * LP_THREADS) {
-                float v[E];
-                LpSpan<T>::unpack(sp.vec(k), v);
+        if (acc.m >= bound) sm.who[atomicAdd(&sm.nwho, 1)] = (uint16_t)tid;
+        __syncthreads();
+        // their vectors, all at once over the block's threads
+        const int each = (sp.nv + LP_THREADS - 1) / LP_THREADS, pairs = sm.nwho * each;
+#pragma unroll 2
+        for (int k = tid; k < pairs; k += LP_THREADS) {
+            const int t = k / each, at = sm.who[t] + (k - t * each) * LP_THREADS;
+            if (at >= sp.nv) continue;
+            float v[E];
+            LpSpan<T>::unpack(sp.vec(at), v);
 #pragma unroll
-                for (int e = 0; e < E; e++) take(clean(v[e]), sp.va + (int64_t)k * E + e);
-            }
+            for (int e = 0; e < E; e++) take(clean(v[e]), sp.va + (int64_t)at * E + e);
         }
         __syncthreads();
     }
@@ -276,8 +338,12 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
             a.top_lp[(int64_t)row * a.top + r] = id >= 0 ? v - Mz - z : -INFINITY;
         };
         if (a.top > 0) {
-            if (n <= LP_CAND) lp_rank(sm, n, a.top, out);
-            else lp_slow(x, p0, p1, a.top, sm, out);
+            if (n <= LP_CAND) {
+                lp_rank(sm, n, a.top, out);
+                if (n < a.top) lp_banned(x, p0, p1, n, a.top, out);
+            } else {
+                lp_slow(x, p0, p1, a.top, sm, out);
+            }
         }
         return;
     }
@@ -294,8 +360,12 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
         mine->id[r] = id;
     };
     if (a.top > 0) {
-        if (n <= LP_CAND) lp_rank(sm, n, a.top, keep);
-        else lp_slow(x, p0, p1, a.top, sm, keep);
+        if (n <= LP_CAND) {
+            lp_rank(sm, n, a.top, keep);
+            for (int r = n + tid; r < a.top; r += LP_THREADS) keep(r, -INFINITY, -1);  // the join looks for banned ones
+        } else {
+            lp_slow(x, p0, p1, a.top, sm, keep);
+        }
     }
     __threadfence();
     __syncthreads();
@@ -337,7 +407,7 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
         const LpPart *p = parts + k / a.top;
         const float v = __ldcg(&p->v[k % a.top]);
         const int32_t id = __ldcg(&p->id[k % a.top]);
-        if (id >= 0 && v >= jb) {
+        if (id >= 0 && v >= jb && v > -INFINITY) {
             const int c = atomicAdd(&sm.n, 1);
             if (c < LP_CAND) {
                 sm.cv[c] = v;
@@ -350,8 +420,13 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
         a.top_ids[(int64_t)row * a.top + r] = id;
         a.top_lp[(int64_t)row * a.top + r] = id >= 0 ? v - jz - z : -INFINITY;
     };
-    if (sm.n <= LP_CAND) lp_rank(sm, sm.n, a.top, out);
-    else lp_slow(x, 0, a.V, a.top, sm, out);
+    const int jn = sm.n;
+    if (jn <= LP_CAND) {
+        lp_rank(sm, jn, a.top, out);
+        if (jn < a.top) lp_banned(x, 0, a.V, jn, a.top, out);
+    } else {
+        lp_slow(x, 0, a.V, a.top, sm, out);
+    }
 }
 
 // Pieces of a row: what fills the GPU at three blocks an SM, of 4 vectors a

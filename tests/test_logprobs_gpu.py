@@ -119,6 +119,20 @@ def test_masked_rows(torch_cuda, V, rows):
         check(got, xx, ids, 8)
 
 
+@pytest.mark.parametrize("kind", list(ACT))
+@pytest.mark.parametrize("V,rows", [(5000, 200), (201088, 2)])
+def test_few_tokens_allowed(torch_cuda, kind, V, rows):
+    """Constrained decoding: 0 to 40 possible tokens, everything else banned."""
+    rng = np.random.default_rng(V)
+    x = np.full((rows, V), -np.inf, np.float32)
+    for r in range(rows):
+        k = r % 41 if rows > 2 else 7 + r * 30
+        x[r, rng.choice(V, k, replace=False)] = rng.integers(-8, 8, k)
+    ids = rng.integers(0, V, (rows, 1))
+    got, xx = run(torch_cuda, x, ids, 32, kind)
+    check(got, xx, ids, 32)
+
+
 def test_plus_infinity_is_nan(torch_cuda):
     x = np.zeros((2, 40), np.float32)
     x[0, 3] = np.inf
