@@ -1,6 +1,11 @@
 // mg_kv4.cu -- storing keys and values in the 4-bit paged cache (with the
 // per-head norms and the rotation of queries and keys on the way), and
 // reading stored positions back.
+#include <string.h>
+
+#include <initializer_list>
+#include <type_traits>
+
 #include "mg_kv4.cuh"
 
 namespace mg {
@@ -32,17 +37,24 @@ struct AppendArgs {
     Kv4 c;
     int n_tok, n_heads;
     const void *q, *k, *v;
-    int64_t ldq, ldk, ldv, ldo, rope_rows;
+    int64_t ldq, ldk, ldv, ldo;
+    int rope_rows;
     const float *q_norm, *k_norm, *cos, *sin;
     float eps;
     const int32_t *seq, *pos;
     void *q_out;
+    int cache_shares;  // blocks of a token that have keys and values
+    bool wide;         // every row, the rotation and the norm weights of 16-byte alignment
 };
 
-// A thread has the dimensions [4 a, 4 a + 4) of a head and their partners
-// half a head up, which the rotation pairs; HD / 8 lanes make a head and 8
-// lanes a scale group.
-constexpr int AP_THREADS = 256;
+// Block = a token and a share of its heads.  A thread has V = 16 bytes of
+// dimensions [V a, V a + V) of a head and their partners half a head up, which
+// the rotation pairs: HD / 2V lanes make a head, 32 / V lanes a scale group.
+// Blocks of queries and blocks of keys and values differ (the latter first:
+// they take longer), so that no block has both.
+// Bound: HBM (rows in, queries out; the codes are a tenth), which takes many
+// threads in flight.
+constexpr int AP_THREADS = 128;
 
 __device__ __forceinline__ float sticky_f32(double x) {
     // toward zero, with the last bit set when inexact: compares with every
@@ -51,93 +63,202 @@ __device__ __forceinline__ float sticky_f32(double x) {
     return (double)f == x ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
 
-template <int HD>
-__device__ __forceinline__ void store4(uint8_t *tile, int p, int d, const float x[4], bool key) {
-    float top = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+// 16 bytes of a row as numbers, and back
+template <typename T>
+__device__ __forceinline__ void numbers(const uint4 &q, float *x) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    if (!tile) return;
+    for (int i = 0; i < 4; i++) {
+        if constexpr (std::is_same<T, float>::value) {
+            x[i] = __uint_as_float(w[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+        } else {
+            x[2 * i] = __uint_as_float(w[i] << 16);
+            x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 packed(const float *x) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (std::is_same<T, float>::value) {
+            w[i] = __float_as_uint(x[i]);
+        } else if constexpr (std::is_same<T, __half>::value) {
+            const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+            w[i] = *reinterpret_cast<const uint32_t *>(&h);
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <int V, bool WIDE, typename T>
+__device__ __forceinline__ void load_v(const T *src, float x[V]) {
+    if constexpr (WIDE) {
+        numbers<T>(__ldg(reinterpret_cast<const uint4 *>(src)), x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = to_f32(src[i]);
+    }
+}
+template <int V, bool WIDE>
+__device__ __forceinline__ void load_f32(const float *src, float x[V]) {
+    if constexpr (WIDE) {
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const float4 v = __ldg(reinterpret_cast<const float4 *>(src + i));
+            x[i] = v.x; x[i + 1] = v.y; x[i + 2] = v.z; x[i + 3] = v.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) x[i] = src[i];
+    }
+}
+template <int V, bool WIDE, typename T>
+__device__ __forceinline__ void store_v(T *dst, const float x[V]) {
+    if constexpr (WIDE) {
+        *reinterpret_cast<uint4 *>(dst) = packed<T>(x);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; i++) dst[i] = from_f32<T>(x[i]);
+    }
+}
+
+// V numbers of dimensions d .. of position p (0..31 of the tile) stored by the
+// lanes of `mask`, whole scale groups of one head
+template <int HD, int V>
+__device__ __forceinline__ void store_codes(uint8_t *tile, int p, int d, const float x[V], bool key, unsigned mask) {
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < V; i++) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+    for (int o = 16 / V; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(mask, top, o));
     const uint32_t sb = kv4_scale(top);
-    const float s = e5m2_f32(sb);
+    const Kv4Mids m(e5m2_f32(sb));
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 4; i++) w |= kv4_code(x[i], s) << (4 * i);
+    for (int i = 0; i < V; i++) w |= kv4_code(x[i], m) << (4 * i);
     const int at = key ? kv4_k_code<HD>(p, d) : kv4_v_code<HD>(p, d);
-    *reinterpret_cast<uint16_t *>(tile + at) = (uint16_t)w;
+    if constexpr (V == 8) {
+        *reinterpret_cast<uint32_t *>(tile + at) = w;
+    } else {  // two lanes' codes together
+        w |= __shfl_xor_sync(mask, w, 1) << 16;
+        if ((d & 7) == 0) *reinterpret_cast<uint32_t *>(tile + at) = w;
+    }
     if ((d & 31) == 0) tile[key ? kv4_k_scale<HD>(p, d >> 5) : kv4_v_scale<HD>(p, d >> 5)] = (uint8_t)sb;
 }
 
-template <int HD, typename T>
-__global__ void __launch_bounds__(AP_THREADS) k_kv4_append(AppendArgs a) {
-    constexpr int L = HD / 8, HALF = HD / 2;
-    const int heads = a.n_heads + 2 * a.c.n_kv;
-    const int64_t unit = ((int64_t)blockIdx.x * AP_THREADS + threadIdx.x) / L;
-    const int d = (threadIdx.x % L) * 4;
-    const int64_t tok64 = unit / heads;
-    bool live = tok64 < a.n_tok;
-    const int tok = live ? (int)tok64 : 0, h = live ? (int)(unit - tok64 * heads) : 0;
-    const int pos = live ? a.pos[tok] : -1, seq = live ? (a.seq ? a.seq[tok] : 0) : 0;
-    live = live && pos >= 0 && pos < a.c.cap && seq >= 0 && seq < a.c.n_seqs && (!a.cos || pos < a.rope_rows);
-    const int kind = h < a.n_heads ? 0 : (h < a.n_heads + a.c.n_kv ? 1 : 2);
-    const int hh = kind == 0 ? h : (kind == 1 ? h - a.n_heads : h - a.n_heads - a.c.n_kv);
-    float x0[4], x1[4];
+template <int HD, typename T, bool QUERIES, bool WIDE>
+__device__ __forceinline__ void append_share(const AppendArgs &a, int share) {
+    constexpr int V = 16 / sizeof(T), HALF = HD / 2, L = HALF / V;
+    const int tok = blockIdx.x, d = (threadIdx.x % L) * V;
+    const int h = (QUERIES ? 0 : a.n_heads) + share * (blockDim.x / L) + threadIdx.x / L;
+    // the lanes of a head; queries keep whole warps
+    const unsigned mask = QUERIES || L == 32 ? ~0u : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
+    const bool live = h < a.n_heads + (QUERIES ? 0 : 2 * a.c.n_kv);
+    if (!QUERIES && !live) return;
+    const int pos = a.pos[tok], seq = a.seq ? a.seq[tok] : 0;
     {
+        const int kind = QUERIES ? 0 : (h < a.n_heads + a.c.n_kv ? 1 : 2);
+        const int hh = kind == 0 ? (live ? h : 0) : (kind == 1 ? h - a.n_heads : h - a.n_heads - a.c.n_kv);
         const T *src = static_cast<const T *>(kind == 0 ? a.q : (kind == 1 ? a.k : a.v)) +
                        (int64_t)tok * (kind == 0 ? a.ldq : (kind == 1 ? a.ldk : a.ldv)) + (int64_t)hh * HD + d;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            x0[i] = live ? to_f32(src[i]) : 0.f;
-            x1[i] = live ? to_f32(src[i + HALF]) : 0.f;
+        float x0[V], x1[V];
+        load_v<V, WIDE>(src, x0);
+        load_v<V, WIDE>(src + HALF, x1);
+        if (pos < 0 || pos >= a.c.cap || seq < 0 || seq >= a.c.n_seqs || (a.cos && pos >= a.rope_rows)) return;
+        const float *nw = kind == 0 ? a.q_norm : (kind == 1 ? a.k_norm : nullptr);
+        const bool turn = a.cos && kind < 2;
+        float co[V], si[V], w0[V], w1[V];
+        if (turn) {
+            load_f32<V, WIDE>(a.cos + (int64_t)pos * HALF + d, co);
+            load_f32<V, WIDE>(a.sin + (int64_t)pos * HALF + d, si);
         }
-    }
-    uint8_t *tile = kind > 0 && live ? a.c.tile(seq, hh, pos >> 5, kv4_tile_bytes(HD)) : nullptr;
-    const float *nw = kind == 0 ? a.q_norm : a.k_norm;
-    double ss = 0.0;
-    if (a.q_norm || a.k_norm) {  // the same for the whole grid
-#pragma unroll
-        for (int i = 0; i < 4; i++) ss += (double)x0[i] * x0[i] + (double)x1[i] * x1[i];
-#pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    }
-    if (kind < 2) {
-        // keys in 64 bits: a key that rounds to the other side of a midpoint
-        // is off by a whole step of its 4 bits
-        double y0[4], y1[4];
-        const double inv = nw ? 1.0 / sqrt(ss / HD + (double)a.eps) : 1.0;
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            y0[i] = nw ? x0[i] * inv * nw[d + i] : x0[i];
-            y1[i] = nw ? x1[i] * inv * nw[d + HALF + i] : x1[i];
-        }
-        if (a.cos && live) {
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const double c = a.cos[(int64_t)pos * HALF + d + i], s = a.sin[(int64_t)pos * HALF + d + i];
-                const double z0 = y0[i] * c - y1[i] * s, z1 = y1[i] * c + y0[i] * s;
-                y0[i] = z0;
-                y1[i] = z1;
-            }
+        if (nw) {
+            load_f32<V, WIDE>(nw + d, w0);
+            load_f32<V, WIDE>(nw + d + HALF, w1);
         }
         if (kind == 0) {
-            if (live) {
-                T *dst = static_cast<T *>(a.q_out) + (int64_t)tok * a.ldo + (int64_t)hh * HD + d;
+            if (nw) {
+                float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    dst[i] = from_f32<T>((float)y0[i]);
-                    dst[i + HALF] = from_f32<T>((float)y1[i]);
+                for (int i = 0; i < V; i++) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+                const float mean = ss * (1.0f / HD) + a.eps;
+                float inv = rsqrtf(mean);  // and a Newton step
+                inv = mean > 0.f && inv < INFINITY ? inv * fmaf(-0.5f * mean * inv, inv, 1.5f) : inv;
+                const float2 i2 = make_float2(inv, inv);
+#pragma unroll
+                for (int i = 0; i < V; i += 2) {
+                    const float2 y0 = mul2(mul2(make_float2(x0[i], x0[i + 1]), i2), make_float2(w0[i], w0[i + 1]));
+                    const float2 y1 = mul2(mul2(make_float2(x1[i], x1[i + 1]), i2), make_float2(w1[i], w1[i + 1]));
+                    x0[i] = y0.x; x0[i + 1] = y0.y;
+                    x1[i] = y1.x; x1[i + 1] = y1.y;
                 }
             }
-        } else {
+            if (turn) {
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                x0[i] = sticky_f32(y0[i]);
-                x1[i] = sticky_f32(y1[i]);
+                for (int i = 0; i < V; i += 2) {
+                    const float2 a0 = make_float2(x0[i], x0[i + 1]), a1 = make_float2(x1[i], x1[i + 1]);
+                    const float2 c = make_float2(co[i], co[i + 1]), s = make_float2(si[i], si[i + 1]);
+                    const float2 z0 = fma2(a0, c, mul2(a1, make_float2(-s.x, -s.y))), z1 = fma2(a1, c, mul2(a0, s));
+                    x0[i] = z0.x; x0[i + 1] = z0.y;
+                    x1[i] = z1.x; x1[i + 1] = z1.y;
+                }
+            }
+            T *dst = static_cast<T *>(a.q_out) + (int64_t)tok * a.ldo + (int64_t)hh * HD + d;
+            if (live) {
+                store_v<V, WIDE>(dst, x0);
+                store_v<V, WIDE>(dst + HALF, x1);
+            }
+            return;
+        }
+        uint8_t *tile = a.c.tile(seq, hh, pos >> 5, kv4_tile_bytes(HD));
+        if (kind == 1) {
+            // keys in 64 bits: a key that rounds to the other side of a midpoint is off by a whole step of its 4 bits
+            double inv = 1.0;
+            if (nw) {
+                double ss = 0.0;
+#pragma unroll
+                for (int i = 0; i < V; i++) ss += (double)x0[i] * x0[i] + (double)x1[i] * x1[i];
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+                inv = 1.0 / sqrt(ss / HD + (double)a.eps);
+            }
+            if (nw || turn) {
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    double y0 = x0[i], y1 = x1[i];
+                    if (nw) {
+                        y0 = y0 * inv * w0[i];
+                        y1 = y1 * inv * w1[i];
+                    }
+                    if (turn) {
+                        const double c = co[i], s = si[i], z = y0 * c - y1 * s;
+                        y1 = y1 * c + y0 * s;
+                        y0 = z;
+                    }
+                    x0[i] = sticky_f32(y0);
+                    x1[i] = sticky_f32(y1);
+                }
             }
         }
+        store_codes<HD, V>(tile, pos & 31, d, x0, kind == 1, mask);
+        store_codes<HD, V>(tile, pos & 31, d + HALF, x1, kind == 1, mask);
     }
-    __syncwarp();
-    store4<HD>(tile, pos & 31, d, x0, kind == 1);
-    store4<HD>(tile, pos & 31, d + HALF, x1, kind == 1);
+}
+
+template <int HD, typename T, bool WIDE>
+__global__ void __launch_bounds__(AP_THREADS, 8) k_kv4_append(AppendArgs a) {
+    if ((int)blockIdx.y < a.cache_shares) append_share<HD, T, false, WIDE>(a, blockIdx.y);
+    else append_share<HD, T, true, WIDE>(a, blockIdx.y - a.cache_shares);
 }
 
 struct ReadArgs {
@@ -146,45 +267,87 @@ struct ReadArgs {
     const int32_t *seq, *pos;
     void *k, *v;
     int64_t ldk, ldv;
+    bool wide;
 };
 
-template <int HD, typename T>
+// thread = eight dimensions of a token's key and value head
+template <int HD, typename T, bool WIDE>
 __global__ void __launch_bounds__(256) k_kv4_read(ReadArgs a) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    const int dim = a.c.n_kv * HD;
-    const int64_t tok = i / dim;
-    if (tok >= a.n_tok) return;
-    const int col = (int)(i - tok * dim), h = col / HD, d = col % HD;
+    constexpr int L = HD / 8;
+    const int per = a.c.n_kv * L;
+    const uint32_t i = blockIdx.x * 256 + threadIdx.x;
+    const uint32_t tok = i / per;
+    if (tok >= (uint32_t)a.n_tok) return;
+    const int r = (int)(i - tok * per), h = r / L, d = (r - h * L) * 8;
     const int pos = a.pos[tok], seq = a.seq ? a.seq[tok] : 0;
-    float kv = 0.f, vv = 0.f;
-    if (pos >= 0 && pos < a.c.cap && seq >= 0 && seq < a.c.n_seqs) {
-        const uint8_t *tile = a.c.tile(seq, h, pos >> 5, kv4_tile_bytes(HD));
-        const int p = pos & 31, sh = (d & 1) * 4;
-        kv = e2m1_f32(tile[kv4_k_code<HD>(p, d)] >> sh) * e5m2_f32(tile[kv4_k_scale<HD>(p, d >> 5)]);
-        vv = e2m1_f32(tile[kv4_v_code<HD>(p, d)] >> sh) * e5m2_f32(tile[kv4_v_scale<HD>(p, d >> 5)]);
+    const bool in = pos >= 0 && pos < a.c.cap && seq >= 0 && seq < a.c.n_seqs;
+    const uint8_t *tile = in ? a.c.tile(seq, h, pos >> 5, kv4_tile_bytes(HD)) : nullptr;
+    const int p = pos & 31;
+#pragma unroll
+    for (int kv = 0; kv < 2; kv++) {
+        T *dst = static_cast<T *>(kv ? a.v : a.k);
+        if (!dst) continue;
+        dst += (int64_t)tok * (kv ? a.ldv : a.ldk) + h * HD + d;
+        uint32_t c[4] = {0u, 0u, 0u, 0u};
+        float s = 0.f;
+        if (in) {
+            e2m1x8_to_h2(*reinterpret_cast<const uint32_t *>(tile + (kv ? kv4_v_code<HD>(p, d) : kv4_k_code<HD>(p, d))), c);
+            s = e5m2_f32(tile[kv ? kv4_v_scale<HD>(p, d >> 5) : kv4_k_scale<HD>(p, d >> 5)]);
+        }
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&c[j]));
+            x[2 * j] = f.x * s;
+            x[2 * j + 1] = f.y * s;
+        }
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int j = 0; j < 8; j += V) store_v<V, WIDE>(dst + j, x + j);
     }
-    if (a.k) static_cast<T *>(a.k)[tok * a.ldk + col] = from_f32<T>(kv);
-    if (a.v) static_cast<T *>(a.v)[tok * a.ldv + col] = from_f32<T>(vv);
 }
 
 template <typename T>
-static int append_t(const AppendArgs &a, int hd, cudaStream_t st) {
-    const int64_t threads = (int64_t)a.n_tok * (a.n_heads + 2 * a.c.n_kv) * (hd / 8);
-    const int64_t blocks = (threads + AP_THREADS - 1) / AP_THREADS;
-    MG_REQUIRE(blocks < (1LL << 31), MG_ERR_ARG, "kv4_append: too many tokens x heads");
-    if (hd == 64) k_kv4_append<64, T><<<(unsigned)blocks, AP_THREADS, 0, st>>>(a);
-    else k_kv4_append<128, T><<<(unsigned)blocks, AP_THREADS, 0, st>>>(a);
+static int append_t(AppendArgs &a, int hd, cudaStream_t st) {
+    // blocks of up to AP_THREADS threads, smaller ones where that leaves the GPU empty
+    const int lanes = hd / 2 / (16 / (int)sizeof(T)), heads = a.n_heads + 2 * a.c.n_kv;
+    int threads = AP_THREADS;
+    while (threads > 64 && (int64_t)a.n_tok * ceil_div((int64_t)heads * lanes, threads) < num_sms()) threads /= 2;
+    a.cache_shares = ceil_div((int64_t)2 * a.c.n_kv * lanes, threads);
+    const dim3 grid(a.n_tok, (unsigned)(a.cache_shares + ceil_div((int64_t)a.n_heads * lanes, threads)));
+    if (hd == 64) {
+        if (a.wide) k_kv4_append<64, T, true><<<grid, threads, 0, st>>>(a);
+        else k_kv4_append<64, T, false><<<grid, threads, 0, st>>>(a);
+    } else {
+        if (a.wide) k_kv4_append<128, T, true><<<grid, threads, 0, st>>>(a);
+        else k_kv4_append<128, T, false><<<grid, threads, 0, st>>>(a);
+    }
     MG_CHECK_LAUNCH();
     return MG_OK;
 }
 template <typename T>
 static int read_t(const ReadArgs &a, int hd, cudaStream_t st) {
-    const int64_t blocks = ((int64_t)a.n_tok * a.c.n_kv * hd + 255) / 256;
-    MG_REQUIRE(blocks < (1LL << 31), MG_ERR_ARG, "kv4_read: too many tokens");
-    if (hd == 64) k_kv4_read<64, T><<<(unsigned)blocks, 256, 0, st>>>(a);
-    else k_kv4_read<128, T><<<(unsigned)blocks, 256, 0, st>>>(a);
+    const int64_t threads = (int64_t)a.n_tok * a.c.n_kv * (hd / 8);
+    MG_REQUIRE(threads < (1LL << 32) - 256, MG_ERR_ARG, "kv4_read: too many tokens");
+    const unsigned blocks = (unsigned)((threads + 255) / 256);
+    if (hd == 64) {
+        if (a.wide) k_kv4_read<64, T, true><<<blocks, 256, 0, st>>>(a);
+        else k_kv4_read<64, T, false><<<blocks, 256, 0, st>>>(a);
+    } else {
+        if (a.wide) k_kv4_read<128, T, true><<<blocks, 256, 0, st>>>(a);
+        else k_kv4_read<128, T, false><<<blocks, 256, 0, st>>>(a);
+    }
     MG_CHECK_LAUNCH();
     return MG_OK;
+}
+
+// every pointer and row stride (in elements of `size` bytes) of 16-byte alignment
+static bool wide_rows(int size, std::initializer_list<const void *> p, std::initializer_list<int64_t> ld) {
+    for (const void *x : p)
+        if (reinterpret_cast<uintptr_t>(x) & 15) return false;
+    for (int64_t l : ld)
+        if ((l * size) & 15) return false;
+    return true;
 }
 
 }  // namespace mg
@@ -224,7 +387,7 @@ extern "C" int mg_kv4_append(const mg_kv4 *c, int act, int n_tok, int n_heads, c
     a.ldk = ldk;
     a.ldv = ldv;
     a.ldo = ldqo;
-    a.rope_rows = rope_rows;
+    a.rope_rows = (int)(rope_rows < 0x7fffffff ? rope_rows : 0x7fffffff);
     a.q_norm = q_norm;
     a.k_norm = k_norm;
     a.cos = rope_cos;
@@ -233,6 +396,9 @@ extern "C" int mg_kv4_append(const mg_kv4 *c, int act, int n_tok, int n_heads, c
     a.seq = tok_seq;
     a.pos = tok_pos;
     a.q_out = q_out;
+    const int size = act == MG_ACT_F32 ? 4 : 2;
+    a.wide = wide_rows(size, {k, v}, {ldk, ldv}) && (n_heads == 0 || wide_rows(size, {q, q_out}, {ldq, ldqo})) &&
+             wide_rows(4, {q_norm, k_norm, rope_cos, rope_sin}, {});
     cudaStream_t st = (cudaStream_t)stream;
     if (act == MG_ACT_F32) return append_t<float>(a, c->head_dim, st);
     if (act == MG_ACT_F16) return append_t<__half>(a, c->head_dim, st);
@@ -255,6 +421,8 @@ extern "C" int mg_kv4_read(const mg_kv4 *c, int act, int n_tok, const int32_t *t
     a.v = v;
     a.ldk = ldk;
     a.ldv = ldv;
+    const int size = act == MG_ACT_F32 ? 4 : 2;
+    a.wide = (!k || wide_rows(size, {k}, {ldk})) && (!v || wide_rows(size, {v}, {ldv}));
     cudaStream_t st = (cudaStream_t)stream;
     if (act == MG_ACT_F32) return read_t<float>(a, c->head_dim, st);
     if (act == MG_ACT_F16) return read_t<__half>(a, c->head_dim, st);

@@ -76,12 +76,23 @@ __device__ __forceinline__ uint32_t kv4_scale(float top) {
 }
 // The nearest e2m1 code of x / s, ties to the even code: |x| against the
 // exact products s x midpoint (s has 3 significant bits, the midpoints 3).
-// s = 0 gives code 0.
-__device__ __forceinline__ uint32_t kv4_code(float x, float s) {
-    const float a = fabsf(x);
-    uint32_t c = (a > 0.25f * s) + (a >= 0.75f * s) + (a > 1.25f * s) + (a >= 1.75f * s) + (a > 2.5f * s) +
-                 (a >= 3.5f * s) + (a > 5.f * s);
-    if (!(s > 0.f)) c = 0;
+// A midpoint below an odd code belongs to the even one under it, so there the
+// comparison is with the next number up; positive floats compare as their
+// bits.  Three comparisons find the code.  s = 0 gives code 0.
+struct Kv4Mids {
+    int32_t m[7];
+    __device__ __forceinline__ explicit Kv4Mids(float s) {
+        const float k[7] = {0.25f, 0.75f, 1.25f, 1.75f, 2.5f, 3.5f, 5.f};
+#pragma unroll
+        for (int i = 0; i < 7; i++) m[i] = s > 0.f ? __float_as_int(k[i] * s) + (i % 2 == 0) : 0x7fffffff;
+    }
+};
+__device__ __forceinline__ uint32_t kv4_code(float x, const Kv4Mids &t) {
+    int32_t a = __float_as_int(x) & 0x7fffffff;
+    a = a > 0x7f800000 ? 0 : a;  // NaN
+    const bool hi = a >= t.m[3], mid = a >= (hi ? t.m[5] : t.m[1]);
+    const int32_t last = hi ? (mid ? t.m[6] : t.m[4]) : (mid ? t.m[2] : t.m[0]);
+    const uint32_t c = (hi ? 4u : 0u) + (mid ? 2u : 0u) + (a >= last ? 1u : 0u);
     return c | (x < 0.f ? 8u : 0u);
 }
 
