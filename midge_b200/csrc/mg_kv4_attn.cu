@@ -42,7 +42,8 @@ namespace mg {
 constexpr int KD_NST = 4;    // ring stages of a warp
 constexpr int KD_ERR = 41;
 constexpr int KD_WARPS_LONG = 4, KD_WARPS_SHORT = 2;  // warps of a block
-constexpr int KD_MIN_CHUNK = 16;                      // tiles worth a piece of their own
+constexpr int KD_MIN_CHUNK = 16;                      // tiles worth a piece of their own where blocks would be idle,
+constexpr int KD_LONG_CHUNK = 64;                     // and where they would not (a piece costs about 16 tiles)
 constexpr int KD_MAX_CUT = 128;                       // pieces of a unit
 __host__ __device__ constexpr int kd_warps_sm(int hd) { return hd == 64 ? 16 : 12; }  // 128 and 168 registers a thread
 
@@ -126,7 +127,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
     sum = 0;
 #pragma unroll
     for (int w = 0; w < KD_WARPS; w++) sum += s_sum[w];
-    const int chunk = (int)max((long long)KD_MIN_CHUNK, div_line(sum + a.pieces - 1, a.pieces));
+    const int chunk = (int)max((long long)a.min_chunk, div_line(sum + a.pieces - 1, a.pieces));
     auto cuts = [&](const Kv4Seq &q) { return min(KD_MAX_CUT, (q.tiles + chunk - 1) / chunk); };
     int2 mine = make_int2(0, 0);  // pieces; pieces of cut units
     for (int s = s0; s < s1; s++) {
@@ -552,7 +553,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
 // there are more of them than blocks of four fit.
 constexpr int KD_WAVES = 4;
 struct FewCut {
-    int blocks, pieces, warps;
+    int blocks, pieces, min_chunk, warps;
 };
 static int few_most(int hd, int warps) { return num_sms() * (kd_warps_sm(hd) / warps); }
 static FewCut few_cut(const Kv4 &c, int gq, int rows, int max_q, int64_t max_kv, int window, int hd) {
@@ -563,8 +564,10 @@ static FewCut few_cut(const Kv4 &c, int gq, int rows, int max_q, int64_t max_kv,
     FewCut f{};
     f.pieces = (int)(units * 4 <= most ? most - units : most * KD_WAVES - (units < most ? units : most));
     f.warps = tiles <= KD_MIN_CHUNK && units > most ? KD_WARPS_SHORT : KD_WARPS_LONG;
+    const int64_t share = units * tiles / most;  // of a block that fits, if there were one piece for each
+    f.min_chunk = (int)(share < KD_MIN_CHUNK ? KD_MIN_CHUNK : share > KD_LONG_CHUNK ? KD_LONG_CHUNK : share);
     int64_t chunk = (units * tiles + f.pieces - 1) / f.pieces;
-    if (chunk < KD_MIN_CHUNK) chunk = KD_MIN_CHUNK;
+    if (chunk < f.min_chunk) chunk = f.min_chunk;
     const int64_t blocks = units * ((tiles + chunk - 1) / chunk);
     f.blocks = (int)(blocks < (1 << 20) ? blocks : 1 << 20);
     return f;
@@ -573,6 +576,7 @@ static FewCut few_cut(const Kv4 &c, int gq, int rows, int max_q, int64_t max_kv,
 template <int HD, int MODE, typename T, int WARPS>
 static int launch_few(Kv4AttnArgs &a, const FewCut &f, cudaStream_t st) {
     a.pieces = f.pieces;
+    a.min_chunk = f.min_chunk;
     TRY(ensure_smem(k_kv4_attn_few<HD, MODE, T, WARPS>, kd_smem<HD>(WARPS)));
     k_kv4_attn_few<HD, MODE, T, WARPS><<<f.blocks, WARPS * 32, kd_smem<HD>(WARPS), st>>>(a);
     MG_CHECK_LAUNCH();

@@ -23,7 +23,7 @@ struct Kv4AttnArgs {
     float *parts;
     unsigned *count;
     int row_groups;   // the most row groups of a sequence
-    int pieces;       // pieces wanted of the whole call
+    int pieces, min_chunk;  // pieces wanted of the whole call, and the least tiles of one
     int *err;
 };
 
