@@ -7,6 +7,8 @@
 // t <= p, with a window also t > p - window:
 //   o = sum_t e^(s_t - m) v_t / (sum_t e^(s_t - m) [+ e^(sink - m)]),  s_t = scale q.k_t
 // and 0 where it sees nothing.  The head h reads key/value head h / gq.
+#include <type_traits>
+
 #include "mg_kernels.h"
 #include "mg_kv4_attn.h"
 #include "mg_tc.cuh"
@@ -67,13 +69,20 @@ __device__ __forceinline__ void split_h2(float a, float b, uint32_t &hi, uint32_
     const __half2 h = __floats2half2_rn(a, b);
     const float2 f = __half22float2(h);
     hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = h2_rn(a - f.x, b - f.y);
+    const float2 r = fma2(f, make_float2(-1.f, -1.f), make_float2(a, b));
+    lo = h2_rn(r.x, r.y);
 }
 // the transpose of an 8 x 8 f16 matrix held as lane (row lane / 4, columns 2 (lane % 4), + 1)
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(x));
     return r;
+}
+// D = A B, nothing added
+__device__ __forceinline__ void mma4_first(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma4(float d[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     const uint32_t a[4] = {a0, a1, a2, a3};
@@ -200,10 +209,9 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
         auto issue = [&](int i) {  // all lanes
             if (i >= wt || !ok) return;
             if (i - addr_base >= 32) look_up(i);
-            const uint64_t p = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(addr), i - addr_base);
-            if (lane == 0) {
+            if (lane == i - addr_base) {
                 mbar_arrive_expect_tx(&bars[warp][i % KD_NST], TB);
-                bulk_g2s(ring + (size_t)(i % KD_NST) * TB, reinterpret_cast<const void *>(p), TB, &bars[warp][i % KD_NST]);
+                bulk_g2s(ring + (size_t)(i % KD_NST) * TB, addr, TB, &bars[warp][i % KD_NST]);
             }
         };
         look_up(0);
@@ -235,8 +243,9 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             // 2^-e, e = the exponent of the row's largest: the row's values are below 2 in f16
             const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
-            const float down = __uint_as_float((254u - e) << 23);
-            own_factor[s] = a.scale * LOG2E * __uint_as_float(e << 23);
+            // (with the scale's sign, so that the factor of the scores is above zero)
+            const float down = __uint_as_float((254u - e) << 23) * (a.scale < 0.f ? -1.f : 1.f);
+            own_factor[s] = fmaxf(fabsf(a.scale) * LOG2E * __uint_as_float(e << 23), 1e-37f);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 const float x0 = x[s][4 * k] * down, x1 = x[s][4 * k + 1] * down;
@@ -251,18 +260,20 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
             }
         }
         // ---- the rows whose scores this lane holds: 8 s + 2 t + c
-        float m[SETS][2], l[SETS][2], factor[SETS][2];
+        float2 m[SETS], l[SETS], factor[SETS];
         int hi[SETS][2];
 #pragma unroll
-        for (int s = 0; s < SETS; s++)
+        for (int s = 0; s < SETS; s++) {
+            factor[s].x = __shfl_sync(0xffffffffu, own_factor[s], 8 * t);
+            factor[s].y = __shfl_sync(0xffffffffu, own_factor[s], 8 * t + 4);
+            m[s] = make_float2(-INFINITY, -INFINITY);
+            l[s] = make_float2(0.f, 0.f);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
-                factor[s][c] = __shfl_sync(0xffffffffu, own_factor[s], (2 * t + c) * 4);
                 const int j = (rg * ROWS + 8 * s + 2 * t + c) / a.gq;
                 hi[s][c] = j < q.nq ? q.before + j : -1;
-                m[s][c] = -INFINITY;
-                l[s][c] = 0.f;
             }
+        }
         float o[SETS][MT][4];  // dimension 2 MT g + 2 mt (+ 1: elements 2, 3), rows 2 t, 2 t + 1
 #pragma unroll
         for (int s = 0; s < SETS; s++)
@@ -271,14 +282,9 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
 #pragma unroll
                 for (int c = 0; c < 4; c++) o[s][i][c] = 0.f;
 
-#pragma unroll 1
-        for (int i = 0; i < wt; i++) {
-            issue(i + KD_NST - 1);  // into the stage that tile i - 1 left
-            const int st = i % KD_NST;
-            ok = ok && mbar_wait(&bars[warp][st], (phase >> st) & 1);
-            phase ^= 1u << st;
-            const uint8_t *tb = ring + (size_t)st * TB;
-            const int p0 = (tile_a + warp + i * KD_WARPS) * 32;
+        // ---- a tile's work
+        auto work = [&](const uint8_t *tb, int p0, auto edge) {
+            constexpr bool EDGE = decltype(edge)::value;
             const uint32_t ksc = *reinterpret_cast<const uint32_t *>(tb + 32 * HD + (g * G + t * G / 4) * 4);
             // ---- scores: sc[s][u][2 j + c] = position 16 u + 2 g + j, row 8 s + 2 t + c
             float sc[SETS][2][4];
@@ -297,8 +303,6 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
                 }
                 const uint32_t f0 = scale_h2(ksc, 2 * u), f1 = scale_h2(ksc, 2 * u + 1);
 #pragma unroll
-                for (int s = 0; s < SETS; s++) sc[s][u][0] = sc[s][u][1] = sc[s][u][2] = sc[s][u][3] = 0.f;
-#pragma unroll
                 for (int w = 0; w < HD / 32; w++) {
                     uint32_t h0[4], h1[4];
                     e2m1x8_to_h2(kw[0][w], h0);
@@ -313,82 +317,81 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
 #pragma unroll
                         for (int s = 0; s < SETS; s++) {
                             const uint32_t *b = qb[s][2 * w + k];
-                            mma4(sc[s][u], h0[2 * k], h1[2 * k], h0[2 * k + 1], h1[2 * k + 1], b[0], b[1]);
+                            if (w == 0 && k == 0) mma4_first(sc[s][u], h0[0], h1[0], h0[1], h1[1], b[0], b[1]);
+                            else mma4(sc[s][u], h0[2 * k], h1[2 * k], h0[2 * k + 1], h1[2 * k + 1], b[0], b[1]);
                             if constexpr (MODE == KD_SPLIT)
                                 mma4(sc[s][u], h0[2 * k], h1[2 * k], h0[2 * k + 1], h1[2 * k + 1], b[2], b[3]);
                         }
                 }
             }
             // ---- weights
-            // some row does not see some position: the last tiles, and with a window the first ones
-            const bool edge = p0 + 32 > q.before + 1 || (a.window > 0 && p0 < q.before + q.nq - a.window);
             uint32_t pb[SETS][2][QR];
-            float alpha[SETS][2];
+            float2 alpha[SETS];
 #pragma unroll
             for (int s = 0; s < SETS; s++) {
-                float mm[2];
-#pragma unroll
-                for (int c = 0; c < 2; c++) {
-                    float top = -INFINITY;
+                if (EDGE) {
 #pragma unroll
                     for (int u = 0; u < 2; u++)
 #pragma unroll
-                        for (int j = 0; j < 2; j++) {
-                            float &v = sc[s][u][2 * j + c];
-                            v *= factor[s][c];
-                            if (edge) {
-                                const int p = p0 + 16 * u + 2 * g + j;
-                                v = p <= hi[s][c] && (a.window == 0 || p > hi[s][c] - a.window) ? v : -INFINITY;
-                            }
-                            top = fmaxf(top, v);
-                        }
+                        for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int x = 4; x < 32; x <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-                    const float mn = fmaxf(m[s][c], top);
-                    mm[c] = mn == -INFINITY ? 0.f : mn;
-                    alpha[s][c] = ex2(m[s][c] - mm[c]);
-                    m[s][c] = mn;
-                    l[s][c] *= alpha[s][c];
+                            for (int c = 0; c < 2; c++) {
+                                const int p = p0 + 16 * u + 2 * g + j;
+                                const bool seen = p <= hi[s][c] && (a.window == 0 || p > hi[s][c] - a.window);
+                                sc[s][u][2 * j + c] = seen ? sc[s][u][2 * j + c] : -INFINITY;
+                            }
                 }
+                float2 top = make_float2(max3(fmaxf(sc[s][0][0], sc[s][0][2]), sc[s][1][0], sc[s][1][2]),
+                                         max3(fmaxf(sc[s][0][1], sc[s][0][3]), sc[s][1][1], sc[s][1][3]));
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) {
+                    top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, x));
+                    top.y = fmaxf(top.y, __shfl_xor_sync(0xffffffffu, top.y, x));
+                }
+                top = mul2(top, factor[s]);
+                const float2 mn = make_float2(fmaxf(m[s].x, top.x), fmaxf(m[s].y, top.y));
+                float2 mm = mn;  // -infinity only where a row has seen nothing yet
+                if (EDGE) mm = make_float2(mn.x == -INFINITY ? 0.f : mn.x, mn.y == -INFINITY ? 0.f : mn.y);
+                alpha[s] = make_float2(ex2(m[s].x - mm.x), ex2(m[s].y - mm.y));
+                m[s] = mn;
+                l[s] = mul2(l[s], alpha[s]);
 #pragma unroll
                 for (int u = 0; u < 2; u++)
 #pragma unroll
                     for (int j = 0; j < 2; j++) {
-                        const float e0 = ex2(sc[s][u][2 * j] - mm[0]), e1 = ex2(sc[s][u][2 * j + 1] - mm[1]);
-                        l[s][0] += e0;
-                        l[s][1] += e1;
+                        const float2 x = fma2(make_float2(sc[s][u][2 * j], sc[s][u][2 * j + 1]), factor[s], make_float2(-mm.x, -mm.y));
+                        const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                        l[s] = add2(l[s], e);
                         if constexpr (MODE == KD_SPLIT) {
                             uint32_t h, r;
-                            split_h2(e0, e1, h, r);
+                            split_h2(e.x, e.y, h, r);
                             pb[s][u][j] = transpose8(h);
                             pb[s][u][2 + j] = transpose8(r);
                         } else {
-                            pb[s][u][j] = transpose8(h2_rn(e0, e1));
+                            pb[s][u][j] = transpose8(h2_rn(e.x, e.y));
                         }
                     }
             }
             if constexpr (MODE != KD_SPLIT) {
                 bool same = true;
 #pragma unroll
-                for (int s = 0; s < SETS; s++) same = same && alpha[s][0] == 1.f && alpha[s][1] == 1.f;
+                for (int s = 0; s < SETS; s++) same = same && alpha[s].x == 1.f && alpha[s].y == 1.f;
                 if (!__all_sync(0xffffffffu, same)) {
 #pragma unroll
                     for (int s = 0; s < SETS; s++)
 #pragma unroll
-                        for (int k = 0; k < MT; k++)
-#pragma unroll
-                            for (int c = 0; c < 4; c++) o[s][k][c] *= alpha[s][c & 1];
+                        for (int k = 0; k < MT; k++) {
+                            const float2 x = mul2(make_float2(o[s][k][0], o[s][k][1]), alpha[s]), y = mul2(make_float2(o[s][k][2], o[s][k][3]), alpha[s]);
+                            o[s][k][0] = x.x; o[s][k][1] = x.y; o[s][k][2] = y.x; o[s][k][3] = y.y;
+                        }
                 }
             }
             // ---- values
-            float d[MT][4];  // f32: this tile's sums
-            if constexpr (MODE == KD_SPLIT)
-#pragma unroll
-                for (int k = 0; k < MT; k++) d[k][0] = d[k][1] = d[k][2] = d[k][3] = 0.f;
+            [[maybe_unused]] float d[MT][4];  // f32: this tile's sums
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 uint32_t vs = *reinterpret_cast<const uint32_t *>(tb + 33 * HD + ((t * G + g * G / 8) * 2 + u) * 4);
-                if (edge) vs = live_bytes(vs, p0 + 16 * u + 4 * t, q.first, q.len);
+                if (EDGE) vs = live_bytes(vs, p0 + 16 * u + 4 * t, q.first, q.len);
                 const uint32_t f02 = __byte_perm(vs, 0u, 0x2404), f13 = __byte_perm(vs, 0u, 0x3414);
                 uint32_t w[4][HD / 64];  // words of positions 4 t + i
                 if constexpr (HD == 64) {
@@ -414,7 +417,8 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
                         const uint32_t a0 = hmul2_u32(e02[k], f02), a1 = hmul2_u32(o02[k], f02);
                         const uint32_t a2 = hmul2_u32(e13[k], f13), a3 = hmul2_u32(o13[k], f13);
                         if constexpr (MODE == KD_SPLIT) {
-                            mma4(d[4 * x + k], a0, a1, a2, a3, pb[0][u][0], pb[0][u][1]);
+                            if (u == 0) mma4_first(d[4 * x + k], a0, a1, a2, a3, pb[0][u][0], pb[0][u][1]);
+                            else mma4(d[4 * x + k], a0, a1, a2, a3, pb[0][u][0], pb[0][u][1]);
                             mma4(d[4 * x + k], a0, a1, a2, a3, pb[0][u][2], pb[0][u][3]);
                         } else {
 #pragma unroll
@@ -423,11 +427,26 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
                     }
                 }
             }
-            if constexpr (MODE == KD_SPLIT)
+            if constexpr (MODE == KD_SPLIT) {
 #pragma unroll
-                for (int k = 0; k < MT; k++)
-#pragma unroll
-                    for (int c = 0; c < 4; c++) o[0][k][c] = fmaf(o[0][k][c], alpha[0][c & 1], d[k][c]);
+                for (int k = 0; k < MT; k++) {
+                    const float2 x = fma2(make_float2(o[0][k][0], o[0][k][1]), alpha[0], make_float2(d[k][0], d[k][1]));
+                    const float2 y = fma2(make_float2(o[0][k][2], o[0][k][3]), alpha[0], make_float2(d[k][2], d[k][3]));
+                    o[0][k][0] = x.x; o[0][k][1] = x.y; o[0][k][2] = y.x; o[0][k][3] = y.y;
+                }
+            }
+        };
+#pragma unroll 1
+        for (int i = 0; i < wt; i++) {
+            issue(i + KD_NST - 1);  // into the stage that tile i - 1 left
+            const int st = i % KD_NST;
+            ok = ok && mbar_wait(&bars[warp][st], (phase >> st) & 1);
+            phase ^= 1u << st;
+            const uint8_t *tb = ring + (size_t)st * TB;
+            const int p0 = (tile_a + warp + i * KD_WARPS) * 32;
+            // some row does not see some position: the last tiles, and with a window the first ones
+            if (p0 + 32 > q.before + 1 || (a.window > 0 && p0 < q.before + q.nq - a.window)) work(tb, p0, std::true_type{});
+            else work(tb, p0, std::false_type{});
             __syncwarp();  // the stage is read: the next issue may fill it
         }
 
@@ -441,11 +460,12 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const int r = 8 * s + 2 * t + c;
+                float sum = c ? l[s].y : l[s].x;
 #pragma unroll
-                for (int x = 4; x < 32; x <<= 1) l[s][c] += __shfl_xor_sync(0xffffffffu, l[s][c], x);
+                for (int x = 4; x < 32; x <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
                 if (g == 0) {
-                    comb[r] = m[s][c];
-                    comb[ROWS + r] = l[s][c];
+                    comb[r] = c ? m[s].y : m[s].x;
+                    comb[ROWS + r] = sum;
                 }
 #pragma unroll
                 for (int k = 0; k < MT; k += 2)
