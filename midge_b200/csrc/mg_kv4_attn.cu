@@ -634,19 +634,22 @@ static int attn_check(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv, K
 }
 
 // Rows of a key/value head from which the tcgen05 kernel (two tiles of 128
-// rows a block) is taken.
-constexpr int KV4_MANY_ROWS = 32;
+// rows a block) is taken.  16 sequences of 4096, us with 48, 64 and 96 rows:
+// few-row kernel 77, 97, 139 (f32, head_dim 64) and 57, 66, 86 (bf16, 128),
+// tcgen05 90, 91, 93 and 57, 58, 59; one sequence of 8192: 17, 20, 24 against
+// 29, 29, 30 and 21, 21, 24 against 31, 31, 32.
+constexpr int KV4_MANY_ROWS = 64;
 static bool is_many(int gq, int max_q) { return (int64_t)gq * max_q > KV4_MANY_ROWS; }
 
 // The workspace: partial results of the most pieces of any call, so that the
 // counters behind them lie in the same place for every call, and a counter
 // per (sequence, key/value head, row group).  Pieces of cut units are at most
 // twice FewCut::pieces (a unit of n > 1 pieces has more than n / 2 chunks);
-// the many-row kernel cuts only as far as all pieces fit the GPU at a time.
+// the many-row kernel has its own bound and no counters.
 static int64_t attn_part_bytes() {
     const int64_t d64 = (int64_t)few_most(64, KD_WARPS_LONG) * kv4_part_floats(16, 64);
     const int64_t d128 = (int64_t)few_most(128, KD_WARPS_LONG) * kv4_part_floats(16, 128);
-    const int64_t few = 2 * KD_WAVES * (d64 > d128 ? d64 : d128) * 4, many = (int64_t)num_sms() * kv4_part_floats(256, 128) * 4;
+    const int64_t few = 2 * KD_WAVES * (d64 > d128 ? d64 : d128) * 4, many = kv4_many_part_floats(num_sms()) * 4;
     return few > many ? few : many;
 }
 static int64_t attn_work(const Kv4 &c, int groups) {
@@ -696,12 +699,7 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
     a.err = stream_error_word();
     MG_REQUIRE(a.err, MG_ERR_OOM, "kv4_attn: no error word");
     cudaStream_t st = (cudaStream_t)stream;
-    if (is_many(a.gq, max_q)) {
-        const int row_tiles = ceil_div((int64_t)max_q * a.gq, 256);
-        int64_t len = window > 0 && max_kv > (int64_t)window + max_q ? (int64_t)window + max_q : max_kv;
-        const int cuts = kv4_many_cuts((int64_t)c->n_seqs * c->n_kv_heads * row_tiles, ceil_div(len, 128));
-        return kv4_attn_many(a, c->head_dim, act, row_tiles, cuts, st);
-    }
+    if (is_many(a.gq, max_q)) return kv4_attn_many(a, c->head_dim, act, max_kv, st);
     const int mode = few_mode(act, a.gq, max_q);
     const FewCut f = few_cut(a.c, a.gq, kd_rows(mode), max_q, max_kv, window, c->head_dim);
     if (act == MG_ACT_F32) return attn_few<float>(a, c->head_dim, mode, f, st);

@@ -79,8 +79,8 @@ template <typename T> __device__ __forceinline__ void store4f(T *dst, bool wide,
     }
 }
 
-// mg_kv4_prompt.cu: blocks of 256 rows; cuts: pieces of a unit
-int kv4_many_cuts(int64_t units, int64_t blocks);
-int kv4_attn_many(const Kv4AttnArgs &a, int hd, int act, int row_tiles, int cuts, cudaStream_t st);
+// mg_kv4_prompt.cu: blocks of 256 rows
+int64_t kv4_many_part_floats(int sms);
+int kv4_attn_many(const Kv4AttnArgs &a, int hd, int act, int64_t max_kv, cudaStream_t st);
 
 }  // namespace mg

@@ -150,6 +150,53 @@ struct KpPieces {
     uint32_t sc[MINE];
 };
 
+// What all blocks (and the join) agree on, from the sequences' lengths; a
+// block's threads together.
+//   chunk  blocks of positions of a piece: a share of a block that fits the GPU
+//          and a quarter more, so that units of one length stay whole and long
+//          ones among short ones do not
+//   order  the sequences, those with the most work first (up to KP_ORDER of them)
+constexpr int KP_MIN = 6, KP_ORDER = 512;
+struct KpPlan {
+    long long part[KP_THREADS / 32];
+    int cost[KP_ORDER];
+    uint16_t order[KP_ORDER];
+    int chunk;
+    bool ordered;
+};
+template <int KVB>
+__device__ __forceinline__ void kp_plan(KpPlan &p, const Kv4AttnArgs &a, int slots, int cuts) {
+    const int n = a.c.n_seqs;
+    const bool ordered = n > 1 && n <= KP_ORDER;
+    long long sum = 0;
+    if (ordered || cuts > 1) {
+        for (int s = threadIdx.x; s < n; s += blockDim.x) {
+            Kv4Seq q;
+            q.load(a, s);
+            const int c = q.nq > 0 ? (q.nq * a.gq + KP_ROWS - 1) / KP_ROWS * ((q.len - (q.first & ~31) + KVB - 1) / KVB) : 0;
+            if (ordered) p.cost[s] = c;
+            sum += (long long)c * a.c.n_kv;
+        }
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if ((threadIdx.x & 31) == 0) p.part[threadIdx.x >> 5] = sum;
+    __syncthreads();
+    if (ordered)
+        for (int s = threadIdx.x; s < n; s += blockDim.x) {
+            int r = 0;
+            for (int k = 0; k < n; k++) r += p.cost[k] > p.cost[s] || (p.cost[k] == p.cost[s] && k < s);
+            p.order[r] = (uint16_t)s;
+        }
+    if (threadIdx.x == 0) {
+        sum = 0;
+        for (int w = 0; w < (int)blockDim.x / 32; w++) sum += p.part[w];
+        p.ordered = ordered;
+        p.chunk = cuts > 1 ? (int)max((long long)KP_MIN * 128 / KVB, (sum * 5 / 4 + slots - 1) / slots) : 1 << 30;
+    }
+    __syncthreads();
+}
+
 // What a block does.  Each role works it out for itself after it has its
 // registers: values that live across setmaxnreg are held to the smaller count
 // and spilled (measured: the softmax twice as slow).
@@ -159,15 +206,16 @@ struct KpUnit {
     int seq, kh, rt, rows, cut, ncut;  // rows from this block's first to the sequence's last
     int nblk, pos0;                    // blocks of positions of this piece, its first position
     int nb[2], first_p[2], last_p[2];  // per tile: blocks it needs, position of its first and last row
-    __device__ __forceinline__ bool load(const Kv4AttnArgs &a, int row_tiles, int cuts) {
-        // later rows first, they see the most; pieces of a unit side by side
-        int u = blockIdx.x;
+    // u: units (the sequences in order, later rows first: they see the most) x pieces, a unit's side by side; a unit has
+    // as many of its `cuts` as pieces of about `chunk` blocks take
+    __device__ __forceinline__ bool load(const Kv4AttnArgs &a, const KpPlan &p, int u, int row_tiles, int cuts) {
         cut = u % cuts;
         u /= cuts;
         kh = u % a.c.n_kv;
         u /= a.c.n_kv;
-        seq = u % a.c.n_seqs;
-        rt = row_tiles - 1 - u / a.c.n_seqs;
+        rt = row_tiles - 1 - u % row_tiles;
+        seq = u / row_tiles;
+        if (p.ordered) seq = p.order[seq];
         q.load(a, seq);
         rows = q.nq * a.gq - rt * KP_ROWS;
         if (rows <= 0) return false;
@@ -180,7 +228,7 @@ struct KpUnit {
             nb[i] = 128 * i < rows ? max(0, (last_p[i] + 1 - start + KVB - 1) / KVB) : 0;
         }
         const int all = max(nb[0], nb[1]);
-        ncut = max(1, min(cuts, all));
+        ncut = max(1, min(cuts, (int)(((long long)all + p.chunk - 1) / p.chunk)));
         if (cut >= ncut) return false;
         const int b0 = (int)((long long)all * cut / ncut), b1 = (int)((long long)all * (cut + 1) / ncut);
         nblk = b1 - b0;
@@ -192,7 +240,7 @@ struct KpUnit {
 };
 
 template <int HD, bool SPLIT, typename T>
-__global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, int row_tiles, int cuts) {
+__global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, int row_tiles, int cuts, int slots, int part_rows) {
     using C = KpCfg<HD, SPLIT>;
     constexpr int KVB = C::KVB, TB = kv4_tile_bytes(HD), G = HD / 32;
     extern __shared__ uint8_t raw_smem[];
@@ -200,13 +248,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     uint8_t *sq = base, *sk = base + 2 * C::Q_TILE, *sv = sk + 2 * C::KV_STAGE;
     __shared__ uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full;
     __shared__ uint32_t tmem_base;
-    __shared__ int s_last;
     __shared__ float s_factor[KP_ROWS];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
+    __shared__ KpPlan plan;
+    kp_plan<KVB>(plan, a, slots, cuts);
     {
         KpUnit<KVB> u;
-        if (!u.load(a, row_tiles, cuts)) return;  // the whole block
+        if (!u.load(a, plan, blockIdx.x, row_tiles, cuts)) return;  // the whole block
     }
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -230,7 +279,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(C::REG_OTHER) : "memory");
         const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(&tmem_base), 0);
         KpUnit<KVB> u;
-        u.load(a, row_tiles, cuts);
+        u.load(a, plan, blockIdx.x, row_tiles, cuts);
         const Kv4Seq &q = u.q;
         const int nblk = u.nblk, pos0 = u.pos0, seq = u.seq, kh = u.kh;
         bool ok = true;
@@ -409,9 +458,9 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(C::REG_SOFTMAX) : "memory");
         const uint32_t tmem = __shfl_sync(0xffffffffu, *reinterpret_cast<volatile uint32_t *>(&tmem_base), 0);
         KpUnit<KVB> u;
-        u.load(a, row_tiles, cuts);
+        u.load(a, plan, blockIdx.x, row_tiles, cuts);
         const Kv4Seq &q = u.q;
-        const int rt = u.rt, kh = u.kh, seq = u.seq, rows = u.rows, cut = u.cut, ncut = u.ncut, pos0 = u.pos0, before = q.before;
+        const int rt = u.rt, kh = u.kh, ncut = u.ncut, pos0 = u.pos0, before = q.before;
         bool ok = true;
         // ---------------------------------------------------- softmax, thread = row
         const int i = warp >> 2, blocks = i ? u.nb[1] : u.nb[0];
@@ -667,48 +716,15 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                     store4f(dst + k, a.out_wide, make_float4(o[k] * f, o[k + 1] * f, o[k + 2] * f, o[k + 3] * f));
             }
         } else {
-            const size_t unit = ((size_t)seq * a.c.n_kv + kh) * row_tiles + rt;
-            constexpr size_t PF = kv4_part_floats(KP_ROWS, HD);
-            float *parts = a.parts + unit * cuts * PF, *part = parts + (size_t)cut * PF;
-            const int rr = 128 * i + r;
-            part[rr] = m;
-            part[KP_ROWS + rr] = l;
+            // for k_kv4_join
+            if (live) {
+                float *part = a.parts + (size_t)blockIdx.x * part_rows * (HD + 2);
+                const int rr = 128 * i + r;
+                part[rr] = m;
+                part[part_rows + rr] = l;
 #pragma unroll
-            for (int k = 0; k < HD; k += 4)
-                *reinterpret_cast<float4 *>(part + 2 * KP_ROWS + (size_t)rr * HD + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
-            __threadfence();
-            named_bar_sync(1, 256);
-            if (tid == 0) {
-                unsigned *cnt = a.count + ((size_t)seq * a.c.n_kv + kh) * a.row_groups + rt;
-                const bool last = atomicAdd(cnt, 1u) + 1u == (unsigned)ncut;
-                if (last) *cnt = 0u;
-                s_last = last;
-                __threadfence();
-            }
-            named_bar_sync(1, 256);
-            if (s_last) {
-                // thread = 4 dimensions of a row
-                for (int x = tid * 4; x < min(rows, KP_ROWS) * HD; x += 256 * 4) {
-                    const int r2 = x / HD, d = x - r2 * HD, row2 = rt * KP_ROWS + r2, j2 = row2 / a.gq;
-                    const int h2 = kh * a.gq + row2 - j2 * a.gq;
-                    const float sk = a.sinks ? a.sinks[h2] * LOG2E : -INFINITY;
-                    float M = sk;
-#pragma unroll 4
-                    for (int c = 0; c < ncut; c++) M = fmaxf(M, __ldcg(parts + c * PF + r2));
-                    const float mm = M == -INFINITY ? 0.f : M;
-                    float L = a.sinks ? kp_ex2(sk - mm) : 0.f;
-                    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int c = 0; c < ncut; c++) {
-                        const float e = kp_ex2(__ldcg(parts + c * PF + r2) - mm);
-                        const float4 v = __ldcg(reinterpret_cast<const float4 *>(parts + c * PF + 2 * KP_ROWS + x));
-                        L += __ldcg(parts + c * PF + KP_ROWS + r2) * e;
-                        acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
-                    }
-                    const float f = L > 0.f ? 1.f / L : 0.f;
-                    store4f(static_cast<T *>(a.out) + (int64_t)(q.q0 + j2) * a.ldo + (int64_t)h2 * HD + d, a.out_wide,
-                            make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
-                }
+                for (int k = 0; k < HD; k += 4)
+                    *reinterpret_cast<float4 *>(part + 2 * part_rows + (size_t)rr * HD + k) = make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]);
             }
         }
     }
@@ -720,14 +736,82 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     }
 }
 
-// pieces of a unit: as many as still fit the GPU at a time, one where the units fill it
-int kv4_many_cuts(int64_t units, int64_t blocks) {
-    const int64_t c = num_sms() / (units > 0 ? units : 1);
-    return (int)(c < 1 ? 1 : (c > blocks ? (blocks < 1 ? 1 : blocks) : c));
+template <int N> __device__ __forceinline__ void load_f(const float *src, float v[N]) {
+    if constexpr (N == 4) {
+        const float4 x = __ldg(reinterpret_cast<const float4 *>(src));
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+        const float2 x = __ldg(reinterpret_cast<const float2 *>(src));
+        v[0] = x.x; v[1] = x.y;
+    }
+}
+
+// The pieces of cut units joined: a warp a row, HD / 32 outputs a lane.
+constexpr int KJ_WARPS = 8;
+template <int HD, int KVB, typename T>
+__global__ void __launch_bounds__(KJ_WARPS * 32) k_kv4_join(Kv4AttnArgs a, int row_tiles, int cuts, int slots, int part_rows) {
+    constexpr int N = HD / 32;
+    __shared__ KpPlan plan;
+    kp_plan<KVB>(plan, a, slots, cuts);
+    const int per = (part_rows + KJ_WARPS - 1) / KJ_WARPS, unit = blockIdx.x / per, lane = threadIdx.x & 31;
+    const int r = (blockIdx.x % per) * KJ_WARPS + (threadIdx.x >> 5);
+    KpUnit<KVB> u;
+    if (!u.load(a, plan, unit * cuts, row_tiles, cuts) || u.ncut == 1) return;
+    if (r >= min(u.rows, part_rows)) return;
+    const int row = u.rt * KP_ROWS + r, j = row / a.gq, h = u.kh * a.gq + row - j * a.gq;
+    const size_t PF = (size_t)part_rows * (HD + 2);
+    const float *parts = a.parts + (size_t)unit * cuts * PF;
+    const float sk = a.sinks ? a.sinks[h] * LOG2E : -INFINITY;
+    float M = sk;
+    for (int c = lane; c < u.ncut; c += 32) M = fmaxf(M, __ldg(parts + c * PF + r));
+    M = warp_max(M);
+    const float mm = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc[N];
+#pragma unroll
+    for (int k = 0; k < N; k++) acc[k] = 0.f;
+#pragma unroll 4
+    for (int c = 0; c < u.ncut; c++) {
+        const float *p = parts + c * PF, e = kp_ex2(__ldg(p + r) - mm);
+        const float *src = p + 2 * part_rows + (size_t)r * HD + lane * N;
+        L += __ldg(p + part_rows + r) * e;
+        float v[N];
+        load_f<N>(src, v);
+#pragma unroll
+        for (int k = 0; k < N; k++) acc[k] += v[k] * e;
+    }
+    L += a.sinks ? kp_ex2(sk - mm) : 0.f;
+    const float f = L > 0.f ? 1.f / L : 0.f;
+    T *dst = static_cast<T *>(a.out) + (int64_t)(u.q.q0 + j) * a.ldo + (int64_t)h * HD + lane * N;
+#pragma unroll
+    for (int k = 0; k < N; k++) dst[k] = from_f32<T>(acc[k] * f);
+}
+
+// How a call may be cut: units (sequence, key/value head, two row tiles) in
+// as many pieces of KP_MIN x 128 positions or more as there are places for
+// their results: the rows of one round of full blocks, and KP_ROUNDS rounds of
+// blocks at most.  kp_plan says on the device how far it is.
+constexpr int KP_ROUNDS = 3;
+int64_t kv4_many_part_floats(int sms) { return (int64_t)sms * KP_ROWS * (128 + 2); }
+struct ManyCut {
+    int row_tiles, cuts, part_rows;
+};
+static ManyCut many_cut(const Kv4AttnArgs &a, int64_t max_kv) {
+    ManyCut m;
+    const int64_t rows = (int64_t)a.max_q * a.gq;
+    m.row_tiles = ceil_div(rows, KP_ROWS);
+    m.part_rows = (int)(rows < KP_ROWS ? (rows + 7) / 8 * 8 : KP_ROWS);
+    int64_t len = a.window > 0 && max_kv > (int64_t)a.window + a.max_q ? (int64_t)a.window + a.max_q : max_kv;
+    const int64_t blocks = len < 1 ? 1 : (len + 127) / 128, units = (int64_t)a.c.n_seqs * a.c.n_kv * m.row_tiles;
+    int64_t pieces = (int64_t)num_sms() * KP_ROWS / m.part_rows;
+    if (pieces > (int64_t)num_sms() * KP_ROUNDS) pieces = (int64_t)num_sms() * KP_ROUNDS;
+    int64_t cuts = pieces / units, most = blocks / KP_MIN;
+    if (cuts > most) cuts = most;
+    m.cuts = (int)(cuts < 1 ? 1 : cuts);
+    return m;
 }
 
 template <int HD, bool SPLIT, typename T>
-static int launch_many(const Kv4AttnArgs &a, int row_tiles, int cuts, cudaStream_t st) {
+static int launch_many(const Kv4AttnArgs &a, const ManyCut &m, cudaStream_t st) {
     using C = KpCfg<HD, SPLIT>;
     TRY(ensure_smem(k_kv4_attn_many<HD, SPLIT, T>, C::SMEM));
     static int regs = 0;  // of a thread at launch
@@ -738,20 +822,26 @@ static int launch_many(const Kv4AttnArgs &a, int row_tiles, int cuts, cudaStream
     }
     MG_REQUIRE(regs * KP_THREADS >= 256 * (C::REG_SOFTMAX + C::REG_OTHER), MG_ERR_CUDA,
                "kv4_attn: built with %d registers a thread, too few for its split", regs);
-    const int64_t blocks = (int64_t)row_tiles * a.c.n_seqs * a.c.n_kv * cuts;
+    const int64_t blocks = (int64_t)m.row_tiles * a.c.n_seqs * a.c.n_kv * m.cuts;
     MG_REQUIRE(blocks < (1LL << 31), MG_ERR_ARG, "kv4_attn: too many rows");
-    k_kv4_attn_many<HD, SPLIT, T><<<(unsigned)blocks, KP_THREADS, C::SMEM, st>>>(a, row_tiles, cuts);
+    k_kv4_attn_many<HD, SPLIT, T><<<(unsigned)blocks, KP_THREADS, C::SMEM, st>>>(a, m.row_tiles, m.cuts, num_sms(), m.part_rows);
     MG_CHECK_LAUNCH();
+    if (m.cuts > 1) {
+        const int64_t join = blocks / m.cuts * ceil_div(m.part_rows, KJ_WARPS);
+        k_kv4_join<HD, C::KVB, T><<<(unsigned)join, KJ_WARPS * 32, 0, st>>>(a, m.row_tiles, m.cuts, num_sms(), m.part_rows);
+        MG_CHECK_LAUNCH();
+    }
     return MG_OK;
 }
 
-int kv4_attn_many(const Kv4AttnArgs &a, int hd, int act, int row_tiles, int cuts, cudaStream_t st) {
+int kv4_attn_many(const Kv4AttnArgs &a, int hd, int act, int64_t max_kv, cudaStream_t st) {
+    const ManyCut m = many_cut(a, max_kv);
     if (act == MG_ACT_F32)
-        return hd == 64 ? launch_many<64, true, float>(a, row_tiles, cuts, st) : launch_many<128, true, float>(a, row_tiles, cuts, st);
+        return hd == 64 ? launch_many<64, true, float>(a, m, st) : launch_many<128, true, float>(a, m, st);
     if (act == MG_ACT_F16)
-        return hd == 64 ? launch_many<64, false, __half>(a, row_tiles, cuts, st) : launch_many<128, false, __half>(a, row_tiles, cuts, st);
-    return hd == 64 ? launch_many<64, false, __nv_bfloat16>(a, row_tiles, cuts, st)
-                    : launch_many<128, false, __nv_bfloat16>(a, row_tiles, cuts, st);
+        return hd == 64 ? launch_many<64, false, __half>(a, m, st) : launch_many<128, false, __half>(a, m, st);
+    return hd == 64 ? launch_many<64, false, __nv_bfloat16>(a, m, st)
+                    : launch_many<128, false, __nv_bfloat16>(a, m, st);
 }
 
 }  // namespace mg
