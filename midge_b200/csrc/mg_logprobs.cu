@@ -6,7 +6,7 @@
 // One pass over the row, 16 bytes a thread at a time: a running maximum, sum
 // and weighted sum per thread (fp32, rescaled when the maximum moves), joined
 // at the end.  The alternatives need no second pass: every thread knows its
-// own maximum, the k-th largest of the block's 32 group maxima is a lower
+// own maximum, the k-th largest of the block's 64 group maxima is a lower
 // bound of the k-th largest entry, and only the threads whose maximum reaches
 // it (a few more than k) have entries to collect again, from L2; the handful
 // of candidates is ranked by counting.  A call of few rows cuts each row over
@@ -21,7 +21,7 @@
 namespace mg {
 
 constexpr int LP_THREADS = 512;
-constexpr int LP_GROUPS = 32, LP_LANES = LP_THREADS / LP_GROUPS;  // groups of 16 lanes, one maximum each
+constexpr int LP_GROUPS = 64, LP_LANES = LP_THREADS / LP_GROUPS;  // groups of 8 lanes, one maximum each
 constexpr int LP_CAND = 1024;                                     // candidates that fit shared memory
 constexpr int LP_UNROLL = 4;                                      // 16-byte loads of a thread in flight
 constexpr int LP_MAX_PARTS = 1024, LP_MAX_ROWS = 512;             // of a call that cuts rows
@@ -157,6 +157,54 @@ struct LpSpan {
     }
 };
 
+// the top-th largest of the block's 64 group maxima (sm.gmax) into sm.bound, by two warps
+__device__ __forceinline__ void lp_bound(LpSmem &sm, int top) {
+    if (threadIdx.x >= LP_GROUPS) return;
+    const float g = sm.gmax[threadIdx.x];
+    int r = 0;
+#pragma unroll 16
+    for (int j = 0; j < LP_GROUPS; j++) {
+        const float o = sm.gmax[j];
+        r += o > g || (o == g && j < (int)threadIdx.x);
+    }
+    if (r == top - 1) sm.bound = g;
+}
+
+// The candidates thinned the way the row was, where there are more than
+// ranking by counting is good for (short rows, whose entries few threads
+// hold): each thread has n / LP_THREADS of them.
+constexpr int LP_MANY = 96;
+__device__ __forceinline__ int lp_thin(LpSmem &sm, int n, int top) {
+    if (n <= LP_MANY) return n;
+    constexpr int K = LP_CAND / LP_THREADS;
+    float v[K], g = -INFINITY;
+    int32_t id[K];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int i = k * LP_THREADS + threadIdx.x;
+        v[k] = i < n ? sm.cv[i] : -INFINITY;
+        id[k] = i < n ? sm.ci[i] : -1;
+        g = fmaxf(g, v[k]);
+    }
+#pragma unroll
+    for (int o = LP_LANES / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
+    if (threadIdx.x % LP_LANES == 0) sm.gmax[threadIdx.x / LP_LANES] = g;
+    if (threadIdx.x == 0) sm.n = 0;
+    __syncthreads();
+    lp_bound(sm, top);
+    __syncthreads();
+    const float bound = sm.bound;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+        if (id[k] >= 0 && v[k] >= bound) {
+            const int c = atomicAdd(&sm.n, 1);
+            sm.cv[c] = v[k];
+            sm.ci[c] = id[k];
+        }
+    __syncthreads();
+    return sm.n;
+}
+
 // With fewer than `top` possible tokens in [a, b) (n of them, ranked already)
 // the next are the first banned ones (-infinity, NaN) by index: warp 0 looks
 // for them from a on, and all but n entries are such.
@@ -266,8 +314,7 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
     for (int o = LP_LANES / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
     if (tid % LP_LANES == 0) sm.gmax[tid / LP_LANES] = g;
     __syncthreads();
-    const float gm = sm.gmax[lane];
-    const float M = warp_max(gm);
+    const float M = warp_max(fmaxf(sm.gmax[lane], sm.gmax[lane + 32]));
     float s = acc.s, w = acc.w;
     lp_move(s, w, acc.r, M == -INFINITY ? 0.f : M);
     s = warp_sum(s);
@@ -276,15 +323,7 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
         sm.red[0][warp] = s;
         sm.red[1][warp] = w;
     }
-    if (warp == 0 && a.top > 0) {
-        int r = 0;
-#pragma unroll
-        for (int j = 0; j < LP_GROUPS; j++) {
-            const float o = __shfl_sync(0xffffffffu, gm, j);
-            r += o > gm || (o == gm && j < lane);
-        }
-        if (r == a.top - 1) sm.bound = gm;
-    }
+    if (a.top > 0) lp_bound(sm, a.top);
     __syncthreads();
     s = w = 0.f;
 #pragma unroll
@@ -322,7 +361,8 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
         }
         __syncthreads();
     }
-    const int n = sm.n;
+    int n = sm.n;
+    if (a.top > 0 && n <= LP_CAND) n = lp_thin(sm, n, a.top);
 
     const float Mz = M == -INFINITY ? 0.f : M;
     if (a.splits == 1) {
@@ -420,7 +460,8 @@ __global__ void __launch_bounds__(LP_THREADS, 3) k_logprobs(LpArgs a) {
         a.top_ids[(int64_t)row * a.top + r] = id;
         a.top_lp[(int64_t)row * a.top + r] = id >= 0 ? v - jz - z : -INFINITY;
     };
-    const int jn = sm.n;
+    int jn = sm.n;
+    if (jn <= LP_CAND) jn = lp_thin(sm, jn, a.top);
     if (jn <= LP_CAND) {
         lp_rank(sm, jn, a.top, out);
         if (jn < a.top) lp_banned(x, 0, a.V, jn, a.top, out);
