@@ -56,10 +56,6 @@ __device__ __forceinline__ int kv4_v_scale(int p, int grp) {
 }
 
 __device__ __forceinline__ float e5m2_f32(uint32_t byte) { return h2f((uint16_t)(byte << 8)); }
-__device__ __forceinline__ float e2m1_f32(uint32_t nib) {
-    const uint32_t h = e2m1x2_to_h2(nib & 15u);
-    return h2f((uint16_t)h);
-}
 
 // The scale of a group of largest magnitude `top`: the least e5m2 value s
 // with 6 s >= top, from 2^-14 (the least normal; anything below half its
@@ -123,11 +119,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 
 // ------------------------------------------------------- activation types
-template <int ACT> struct Act;
-template <> struct Act<MG_ACT_F32> { using T = float; };
-template <> struct Act<MG_ACT_F16> { using T = __half; };
-template <> struct Act<MG_ACT_BF16> { using T = __nv_bfloat16; };
-
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }

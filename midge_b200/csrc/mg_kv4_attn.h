@@ -40,7 +40,7 @@ struct Kv4Seq {
         nq = min(n, a.max_q);
         len = (int)min((int64_t)max(l, 0), a.c.cap);
         before = len - n;
-        first = a.window > 0 ? max(0, before - a.window + 1) : 0;
+        first = a.window > 0 ? (int)max(0LL, (long long)before - a.window + 1) : 0;
         tile0 = first >> 5;
         // at least one tile where there is a query, so that its zeros are written
         tiles = nq <= 0 ? 0 : max(1, ((len + 31) >> 5) - tile0);

@@ -219,7 +219,7 @@ struct KpUnit {
         q.load(a, seq);
         rows = q.nq * a.gq - rt * KP_ROWS;
         if (rows <= 0) return false;
-        const int start = a.window > 0 ? max(0, q.before + rt * KP_ROWS / a.gq - a.window + 1) & ~31 : 0;
+        const int start = a.window > 0 ? (int)max(0LL, (long long)q.before + rt * KP_ROWS / a.gq - a.window + 1) & ~31 : 0;
 #pragma unroll
         for (int i = 0; i < 2; i++) {
             const int r0 = rt * KP_ROWS + 128 * i, r1 = min(r0 + 127, q.nq * a.gq - 1);
@@ -468,7 +468,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
         const int r = tid & 127, row = rt * KP_ROWS + 128 * i + r;
         const int j = row / a.gq, h = kh * a.gq + row - j * a.gq;
         const bool live = j < q.nq;
-        const int hi = live ? before + j : -1, lo = a.window > 0 ? hi - a.window + 1 : 0;
+        const int hi = live ? before + j : -1, lo = a.window > 0 ? max(0, hi - a.window + 1) : 0;
         {   // the queries, scaled to below 2 by a power of two per row, into the swizzled tile; the scale's sign goes with
             // them.  A row takes HD / 8 lanes, a lane one 16-byte chunk of the tile.
             constexpr int L = HD / 8, STEP = 32 / L, N = 32 / STEP;
