@@ -206,10 +206,14 @@ int mg_kv4_read(const mg_kv4 *c, int act, int n_tok, const int32_t *tok_seq, con
  * gets zeros.  max_q >= every number of queries (rows beyond it are not
  * written) and max_kv, about the longest kv_len, choose the kernel and its
  * split; any kv_len up to ld_table * page_size is right.
- * work: mg_kv4_attn_work() bytes of device memory, zero before its first use;
- * a call leaves it ready for the next on the same stream, of whatever
- * sizes it is large enough for.  Calls that overlap in time need a workspace
- * each. */
+ * work: mg_kv4_attn_work() bytes of device memory (never 0), 16-byte aligned,
+ * zero before its first use; a call leaves it ready for the next on the same
+ * stream, of whatever sizes it is large enough for.  Calls that overlap in
+ * time need a workspace each.  A call launches one or two kernels, allocates
+ * nothing and waits for nothing, so it may be captured in a CUDA graph; the
+ * first call of a process on a device sets kernel attributes and allocates the
+ * library's error word, so it comes before any capture.  Results do not depend
+ * on the order in which blocks run: the same call gives the same bits. */
 int64_t mg_kv4_attn_work(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv);
 int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q, int64_t ldq, const int32_t *q_start,
                 const int32_t *kv_len, int max_q, int64_t max_kv, float scale, int window, const float *sinks,
@@ -222,8 +226,9 @@ int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q, int64_t ld
  * probabilities, by value and then by index (with V < n_alt the rest is -1
  * and -infinity).  A logit of -infinity has probability 0 and may be an
  * alternative; NaN counts as -infinity.  A row of nothing but -infinity has
- * log probabilities -infinity and entropy 0; one with +infinity has NaN.  lp [n_rows x n_ids], entropy
- * [n_rows], alt_ids / alt_lp [n_rows x n_alt].  work as for mg_kv4_attn. */
+ * log probabilities -infinity and entropy 0; one with +infinity has NaN.
+ * lp [n_rows x n_ids], entropy [n_rows], alt_ids / alt_lp [n_rows x n_alt].
+ * work: mg_logprobs_work() bytes, and otherwise as for mg_kv4_attn. */
 #define MG_LOGPROBS_MAX_ALT 32
 int64_t mg_logprobs_work(int64_t V, int n_rows, int n_alt);
 int mg_logprobs(int act, const void *logits, int64_t ldl, int64_t V, int n_rows, const int32_t *ids, int n_ids,

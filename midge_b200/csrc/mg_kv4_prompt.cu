@@ -5,20 +5,31 @@
 // A block has 256 rows ((query, head) pairs of one key/value head, two tiles
 // of 128) and walks the cache in blocks of KVB positions:
 //   warps 0-3, 4-7    softmax of tile 0 / 1, thread = row: S from TMEM, row
-//                     maximum, weights as f16 back into TMEM over S, the
-//                     products of the last block added to O in registers
+//                     maximum, weights as f16 back into TMEM over S
 //   warps 8-14        codes -> f16 K and V tiles in 128-byte-swizzled shared
 //                     memory (cvt.f16x2.e2m1x2 and the scale: exact), once
 //                     for both tiles
-//   warp 15           one thread issues the MMAs: S = Q K^T (both from shared
-//                     memory), O_block = P V (P from TMEM)
+//   warp 15           issues the MMAs: S = Q K^T (both from shared memory),
+//                     O += P V (P from TMEM)
 // The two tiles alternate: while one tile's MMAs run the other's softmax has
-// the MUFU, which bounds the kernel (16 ex2 per cycle and SM against 4096
-// multiply-adds: at head_dim 64 the exponentials take twice the MMAs' time).
-// O stays in registers in fp32 and each block's product starts from zero: the
-// tensor core truncates its running sum.  f32 rows go as f16 hi + lo, queries
-// and weights (two MMAs each, 22 bits); f16 and bf16 queries are exact in f16
-// after scaling by a power of two per row.
+// the MUFU (16 ex2 per cycle and SM, so 2048 cycles for 256 x 128 weights;
+// the MMAs of the same take some 500 for S and 700 for P V at head_dim 64, twice
+// that in f32).
+// f32: queries and weights go as f16 hi + lo, two MMAs each (22 bits), and O
+// stays in registers: each block's product starts from zero and is added in
+// fp32, since the tensor core truncates its running sum.  f16 and bf16: a
+// query is exact in f16 after scaling by a power of two per row (what falls
+// below f16's range is 2^-24 of the row's largest), weights are rounded to
+// f16 (2^-11, below the result's own rounding in bf16 and like it in f16)
+// and O accumulates in TMEM, whose truncated sums are far finer than either.
+//
+// Measured, one sequence of 4096 new tokens, 64 heads of 64 over 8, f32:
+// 0.36 ms = 380 TFLOP/s, 760 of f16 MMAs; 3 x 1009 tokens behind 5k to 16k,
+// 32 heads of 128 over 4, bf16: 0.51 ms = 1.0 PFLOP/s.  A block of 128 positions
+// takes some 4500 cycles: bound by the chain S -> maximum -> weights -> P V of
+// a tile, of which the other tile hides about half, then by the MUFU; a block
+// of rows adds some 10 us of its own at start and end.  Blocks of 64 positions
+// measured 6% slower on the first and 24% on the second.
 #include <type_traits>
 
 #include "mg_kernels.h"
@@ -151,7 +162,9 @@ struct KpPieces {
 };
 
 // What all blocks (and the join) agree on, from the sequences' lengths; a
-// block's threads together.
+// block's threads together.  Sequences with the most work first and pieces by
+// the call's own length, not by the host's hint: three sequences of 5k to 16k
+// 512 us, in their own order 595.
 //   chunk  blocks of positions of a piece: a share of a block that fits the GPU
 //          and a quarter more, so that units of one length stay whole and long
 //          ones among short ones do not
@@ -746,7 +759,10 @@ template <int N> __device__ __forceinline__ void load_f(const float *src, float 
     }
 }
 
-// The pieces of cut units joined: a warp a row, HD / 32 outputs a lane.
+// The pieces of cut units joined: a warp a row, HD / 32 outputs a lane, in
+// piece order.  Bound: the pieces' bytes from L2 (a launch's 2 to 4 us); in
+// the last piece to finish, as the few-row kernel joins, one block would read
+// 256 rows of every piece.
 constexpr int KJ_WARPS = 8;
 template <int HD, int KVB, typename T>
 __global__ void __launch_bounds__(KJ_WARPS * 32) k_kv4_join(Kv4AttnArgs a, int row_tiles, int cuts, int slots, int part_rows) {

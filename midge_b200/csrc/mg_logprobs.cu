@@ -11,7 +11,12 @@
 // it (a few more than k) have entries to collect again, from L2; the handful
 // of candidates is ranked by counting.  A call of few rows cuts each row over
 // several blocks and the last one to finish joins them, in block order.
-// Bound: HBM (one read of the logits).
+// Bound: HBM (one read of the logits).  Measured: 2047 rows of 151936 bf16, 20
+// alternatives: 138 us (622 MB, 4.5 TB/s); what is missing is each row's end
+// (joins and ranking, some 3 us with three blocks an SM to cover it) and the
+// exponentials.  8 rows of 201088 f32, 5 alternatives: 11 us, a launch, one
+// round of loads and the join of the row's pieces.  Rows that are nearly all
+// one number have more candidates than fit and take a pass per alternative.
 #include <string.h>
 
 #include <type_traits>
