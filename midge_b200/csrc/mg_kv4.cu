@@ -54,11 +54,12 @@ struct AppendArgs {
 // they take longer), so that no block has both.
 // Bound: HBM (rows in, queries out; the codes are a tenth), which takes many
 // threads in flight.  Measured with the read back: 4096 tokens, 64 + 2 x 8 heads
-// of 64, f32: 40 us (165 MB, 4.1 TB/s); 8191 tokens, 32 + 2 x 4 heads of 128 with
-// norms, bf16: 60 us (181 MB, 3.0 TB/s: the norms and the keys' 64-bit arithmetic
-// share the issue slots); 8 tokens: 5.4 us, two launches of two dependent loads.
-// Four elements a thread with queries and keys in the same blocks: 68 and 132 us.
-constexpr int AP_THREADS = 128;
+// of 64, f32: 36.5 us (165 MB, 4.5 TB/s); 8191 tokens, 32 + 2 x 4 heads of 128
+// with norms, bf16: 50 us (181 MB, 3.6 TB/s: the norms and the keys' 64-bit
+// arithmetic share the issue slots); 8 tokens: 5.2 us, two launches of two
+// dependent loads.  A query head a thread: 39 and 59 us, three or four heads 36
+// and 63 or more (16-bit rows spill).
+constexpr int AP_THREADS = 128, AP_HEADS = 2;
 
 __device__ __forceinline__ float sticky_f32(double x) {
     // toward zero, with the last bit set when inexact: compares with every
@@ -158,111 +159,142 @@ __device__ __forceinline__ void store_codes(uint8_t *tile, int p, int d, const f
     if ((d & 31) == 0) tile[key ? kv4_k_scale<HD>(p, d >> 5) : kv4_v_scale<HD>(p, d >> 5)] = (uint8_t)sb;
 }
 
-template <int HD, typename T, bool QUERIES, bool WIDE>
-__device__ __forceinline__ void append_share(const AppendArgs &a, int share) {
+// Queries of a token: a thread has its dimensions of AP_HEADS heads, with one
+// load of the rotation and the weights for all.
+template <int HD, typename T, bool WIDE>
+__device__ __forceinline__ void append_queries(const AppendArgs &a, int share) {
+    constexpr int V = 16 / sizeof(T), HALF = HD / 2, L = HALF / V;
+    const int tok = blockIdx.x, d = (threadIdx.x % L) * V, step = blockDim.x / L;
+    const int h0 = share * step * AP_HEADS + threadIdx.x / L;
+    const int pos = a.pos[tok], seq = a.seq ? a.seq[tok] : 0;
+    const T *src = static_cast<const T *>(a.q) + (int64_t)tok * a.ldq + d;
+    float x0[AP_HEADS][V], x1[AP_HEADS][V];
+#pragma unroll
+    for (int k = 0; k < AP_HEADS; k++) {
+        const int h = min(h0 + k * step, a.n_heads - 1);
+        load_v<V, WIDE>(src + (int64_t)h * HD, x0[k]);
+        load_v<V, WIDE>(src + (int64_t)h * HD + HALF, x1[k]);
+    }
+    if (pos < 0 || pos >= a.c.cap || seq < 0 || seq >= a.c.n_seqs || (a.cos && pos >= a.rope_rows)) return;
+    if (a.q_norm) {
+        float w0[V], w1[V];
+        load_f32<V, WIDE>(a.q_norm + d, w0);
+        load_f32<V, WIDE>(a.q_norm + d + HALF, w1);
+#pragma unroll
+        for (int k = 0; k < AP_HEADS; k++) {
+            float2 s2 = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < V; i++) {
+                const float2 v = make_float2(x0[k][i], x1[k][i]);
+                s2 = fma2(v, v, s2);
+            }
+            float ss = s2.x + s2.y;
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+            const float mean = ss * (1.0f / HD) + a.eps;
+            float inv = rsqrtf(mean);  // and a Newton step
+            inv = mean > 0.f && inv < INFINITY ? inv * fmaf(-0.5f * mean * inv, inv, 1.5f) : inv;
+            const float2 i2 = make_float2(inv, inv);
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const float2 y0 = mul2(mul2(make_float2(x0[k][i], x0[k][i + 1]), i2), make_float2(w0[i], w0[i + 1]));
+                const float2 y1 = mul2(mul2(make_float2(x1[k][i], x1[k][i + 1]), i2), make_float2(w1[i], w1[i + 1]));
+                x0[k][i] = y0.x; x0[k][i + 1] = y0.y;
+                x1[k][i] = y1.x; x1[k][i + 1] = y1.y;
+            }
+        }
+    }
+    if (a.cos) {
+        float co[V], si[V];
+        load_f32<V, WIDE>(a.cos + (int64_t)pos * HALF + d, co);
+        load_f32<V, WIDE>(a.sin + (int64_t)pos * HALF + d, si);
+#pragma unroll
+        for (int k = 0; k < AP_HEADS; k++)
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const float2 a0 = make_float2(x0[k][i], x0[k][i + 1]), a1 = make_float2(x1[k][i], x1[k][i + 1]);
+                const float2 c = make_float2(co[i], co[i + 1]), s = make_float2(si[i], si[i + 1]);
+                const float2 z0 = fma2(a0, c, mul2(a1, make_float2(-s.x, -s.y))), z1 = fma2(a1, c, mul2(a0, s));
+                x0[k][i] = z0.x; x0[k][i + 1] = z0.y;
+                x1[k][i] = z1.x; x1[k][i + 1] = z1.y;
+            }
+    }
+    T *dst = static_cast<T *>(a.q_out) + (int64_t)tok * a.ldo + d;
+#pragma unroll
+    for (int k = 0; k < AP_HEADS; k++) {
+        const int h = h0 + k * step;
+        if (h < a.n_heads) {
+            store_v<V, WIDE>(dst + (int64_t)h * HD, x0[k]);
+            store_v<V, WIDE>(dst + (int64_t)h * HD + HALF, x1[k]);
+        }
+    }
+}
+
+// Keys and values of a token: whole scale groups of a head, the lanes of `mask`.
+template <int HD, typename T, bool WIDE>
+__device__ __forceinline__ void append_cache(const AppendArgs &a, int share) {
     constexpr int V = 16 / sizeof(T), HALF = HD / 2, L = HALF / V;
     const int tok = blockIdx.x, d = (threadIdx.x % L) * V;
-    const int h = (QUERIES ? 0 : a.n_heads) + share * (blockDim.x / L) + threadIdx.x / L;
-    // the lanes of a head; queries keep whole warps
-    const unsigned mask = QUERIES || L == 32 ? ~0u : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
-    const bool live = h < a.n_heads + (QUERIES ? 0 : 2 * a.c.n_kv);
-    if (!QUERIES && !live) return;
+    const int h = share * (blockDim.x / L) + threadIdx.x / L;
+    const unsigned mask = L == 32 ? ~0u : ((1u << L) - 1u) << ((threadIdx.x & 31) / L * L);
+    if (h >= 2 * a.c.n_kv) return;
     const int pos = a.pos[tok], seq = a.seq ? a.seq[tok] : 0;
-    {
-        const int kind = QUERIES ? 0 : (h < a.n_heads + a.c.n_kv ? 1 : 2);
-        const int hh = kind == 0 ? (live ? h : 0) : (kind == 1 ? h - a.n_heads : h - a.n_heads - a.c.n_kv);
-        const T *src = static_cast<const T *>(kind == 0 ? a.q : (kind == 1 ? a.k : a.v)) +
-                       (int64_t)tok * (kind == 0 ? a.ldq : (kind == 1 ? a.ldk : a.ldv)) + (int64_t)hh * HD + d;
-        float x0[V], x1[V];
-        load_v<V, WIDE>(src, x0);
-        load_v<V, WIDE>(src + HALF, x1);
-        if (pos < 0 || pos >= a.c.cap || seq < 0 || seq >= a.c.n_seqs || (a.cos && pos >= a.rope_rows)) return;
-        const float *nw = kind == 0 ? a.q_norm : (kind == 1 ? a.k_norm : nullptr);
-        const bool turn = a.cos && kind < 2;
-        float co[V], si[V], w0[V], w1[V];
-        if (turn) {
-            load_f32<V, WIDE>(a.cos + (int64_t)pos * HALF + d, co);
-            load_f32<V, WIDE>(a.sin + (int64_t)pos * HALF + d, si);
+    const bool key = h < a.c.n_kv;
+    const int hh = key ? h : h - a.c.n_kv;
+    const T *src = static_cast<const T *>(key ? a.k : a.v) + (int64_t)tok * (key ? a.ldk : a.ldv) + (int64_t)hh * HD + d;
+    float x0[V], x1[V];
+    load_v<V, WIDE>(src, x0);
+    load_v<V, WIDE>(src + HALF, x1);
+    if (pos < 0 || pos >= a.c.cap || seq < 0 || seq >= a.c.n_seqs || (a.cos && pos >= a.rope_rows)) return;
+    uint8_t *tile = a.c.tile(seq, hh, pos >> 5, kv4_tile_bytes(HD));
+    if (key && (a.k_norm || a.cos)) {
+        // keys in 64 bits: a key that rounds to the other side of a midpoint is off by a whole step of its 4 bits
+        double inv = 1.0;
+        if (a.k_norm) {
+            double ss = 0.0;
+#pragma unroll
+            for (int i = 0; i < V; i++) ss += (double)x0[i] * x0[i] + (double)x1[i] * x1[i];
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+            inv = 1.0 / sqrt(ss / HD + (double)a.eps);
         }
-        if (nw) {
-            load_f32<V, WIDE>(nw + d, w0);
-            load_f32<V, WIDE>(nw + d + HALF, w1);
-        }
-        if (kind == 0) {
-            if (nw) {
-                float ss = 0.f;
 #pragma unroll
-                for (int i = 0; i < V; i++) ss = fmaf(x0[i], x0[i], fmaf(x1[i], x1[i], ss));
+        for (int j = 0; j < V; j += 4) {  // four at a time: 64-bit values of all would not fit the registers
+            float co[4], si[4], w0[4], w1[4];
+            if (a.cos) {
+                load_f32<4, WIDE>(a.cos + (int64_t)pos * HALF + d + j, co);
+                load_f32<4, WIDE>(a.sin + (int64_t)pos * HALF + d + j, si);
+            }
+            if (a.k_norm) {
+                load_f32<4, WIDE>(a.k_norm + d + j, w0);
+                load_f32<4, WIDE>(a.k_norm + d + HALF + j, w1);
+            }
 #pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-                const float mean = ss * (1.0f / HD) + a.eps;
-                float inv = rsqrtf(mean);  // and a Newton step
-                inv = mean > 0.f && inv < INFINITY ? inv * fmaf(-0.5f * mean * inv, inv, 1.5f) : inv;
-                const float2 i2 = make_float2(inv, inv);
-#pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    const float2 y0 = mul2(mul2(make_float2(x0[i], x0[i + 1]), i2), make_float2(w0[i], w0[i + 1]));
-                    const float2 y1 = mul2(mul2(make_float2(x1[i], x1[i + 1]), i2), make_float2(w1[i], w1[i + 1]));
-                    x0[i] = y0.x; x0[i + 1] = y0.y;
-                    x1[i] = y1.x; x1[i + 1] = y1.y;
+            for (int i = 0; i < 4; i++) {
+                double y0 = x0[j + i], y1 = x1[j + i];
+                if (a.k_norm) {
+                    y0 = y0 * inv * w0[i];
+                    y1 = y1 * inv * w1[i];
                 }
-            }
-            if (turn) {
-#pragma unroll
-                for (int i = 0; i < V; i += 2) {
-                    const float2 a0 = make_float2(x0[i], x0[i + 1]), a1 = make_float2(x1[i], x1[i + 1]);
-                    const float2 c = make_float2(co[i], co[i + 1]), s = make_float2(si[i], si[i + 1]);
-                    const float2 z0 = fma2(a0, c, mul2(a1, make_float2(-s.x, -s.y))), z1 = fma2(a1, c, mul2(a0, s));
-                    x0[i] = z0.x; x0[i + 1] = z0.y;
-                    x1[i] = z1.x; x1[i + 1] = z1.y;
+                if (a.cos) {
+                    const double c = co[i], s = si[i], z = y0 * c - y1 * s;
+                    y1 = y1 * c + y0 * s;
+                    y0 = z;
                 }
+                x0[j + i] = sticky_f32(y0);
+                x1[j + i] = sticky_f32(y1);
             }
-            T *dst = static_cast<T *>(a.q_out) + (int64_t)tok * a.ldo + (int64_t)hh * HD + d;
-            if (live) {
-                store_v<V, WIDE>(dst, x0);
-                store_v<V, WIDE>(dst + HALF, x1);
-            }
-            return;
+            if (V > 4) __syncwarp(mask);
         }
-        uint8_t *tile = a.c.tile(seq, hh, pos >> 5, kv4_tile_bytes(HD));
-        if (kind == 1) {
-            // keys in 64 bits: a key that rounds to the other side of a midpoint is off by a whole step of its 4 bits
-            double inv = 1.0;
-            if (nw) {
-                double ss = 0.0;
-#pragma unroll
-                for (int i = 0; i < V; i++) ss += (double)x0[i] * x0[i] + (double)x1[i] * x1[i];
-#pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-                inv = 1.0 / sqrt(ss / HD + (double)a.eps);
-            }
-            if (nw || turn) {
-#pragma unroll
-                for (int i = 0; i < V; i++) {
-                    double y0 = x0[i], y1 = x1[i];
-                    if (nw) {
-                        y0 = y0 * inv * w0[i];
-                        y1 = y1 * inv * w1[i];
-                    }
-                    if (turn) {
-                        const double c = co[i], s = si[i], z = y0 * c - y1 * s;
-                        y1 = y1 * c + y0 * s;
-                        y0 = z;
-                    }
-                    x0[i] = sticky_f32(y0);
-                    x1[i] = sticky_f32(y1);
-                }
-            }
-        }
-        store_codes<HD, V>(tile, pos & 31, d, x0, kind == 1, mask);
-        store_codes<HD, V>(tile, pos & 31, d + HALF, x1, kind == 1, mask);
     }
+    store_codes<HD, V>(tile, pos & 31, d, x0, key, mask);
+    store_codes<HD, V>(tile, pos & 31, d + HALF, x1, key, mask);
 }
 
 template <int HD, typename T, bool WIDE>
 __global__ void __launch_bounds__(AP_THREADS, 8) k_kv4_append(AppendArgs a) {
-    if ((int)blockIdx.y < a.cache_shares) append_share<HD, T, false, WIDE>(a, blockIdx.y);
-    else append_share<HD, T, true, WIDE>(a, blockIdx.y - a.cache_shares);
+    if ((int)blockIdx.y < a.cache_shares) append_cache<HD, T, WIDE>(a, blockIdx.y);
+    else append_queries<HD, T, WIDE>(a, blockIdx.y - a.cache_shares);
 }
 
 struct ReadArgs {
@@ -318,7 +350,7 @@ static int append_t(AppendArgs &a, int hd, cudaStream_t st) {
     int threads = AP_THREADS;
     while (threads > 64 && (int64_t)a.n_tok * ceil_div((int64_t)heads * lanes, threads) < num_sms()) threads /= 2;
     a.cache_shares = ceil_div((int64_t)2 * a.c.n_kv * lanes, threads);
-    const dim3 grid(a.n_tok, (unsigned)(a.cache_shares + ceil_div((int64_t)a.n_heads * lanes, threads)));
+    const dim3 grid(a.n_tok, (unsigned)(a.cache_shares + ceil_div((int64_t)ceil_div(a.n_heads, AP_HEADS) * lanes, threads)));
     if (hd == 64) {
         if (a.wide) k_kv4_append<64, T, true><<<grid, threads, 0, st>>>(a);
         else k_kv4_append<64, T, false><<<grid, threads, 0, st>>>(a);
