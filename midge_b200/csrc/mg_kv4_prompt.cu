@@ -24,7 +24,7 @@
 // and O accumulates in TMEM, whose truncated sums are far finer than either.
 //
 // Measured, one sequence of 4096 new tokens, 64 heads of 64 over 8, f32:
-// 0.36 ms = 380 TFLOP/s, 760 of f16 MMAs; 3 x 1009 tokens behind 5k to 16k,
+// 0.34 ms = 405 TFLOP/s, 810 of f16 MMAs; 3 x 1009 tokens behind 5k to 16k,
 // 32 heads of 128 over 4, bf16: 0.51 ms = 1.0 PFLOP/s.  A block of 128 positions
 // takes some 4500 cycles: bound by the chain S -> maximum -> weights -> P V of
 // a tile, of which the other tile hides about half, then by the MUFU; a block
@@ -52,6 +52,9 @@ struct KpCfg {
     static constexpr int KV_STAGE = PLANES * KVB * 128;        // bytes of a K (or V) stage
     static constexpr int SMEM = 2 * Q_TILE + 4 * KV_STAGE + 1024;
     static constexpr int TM_S = KVB, TM_O = HD;                // TMEM columns of a tile
+    // products of alternate blocks in places of their own where TMEM has them: they are added after the next weights are out
+    // (4096 tokens, 64 heads of 64, f32: 340 us, with one place 361)
+    static constexpr int O_BUF = SPLIT && 2 * KVB + 4 * HD <= 512 ? 2 : 1;
     static constexpr int CH = SPLIT ? 16 : 32;                 // positions whose weights lie together in TMEM
     // registers of the softmax warps, of the others: two warpgroups of each out of 512 x 128; launch_many checks that the
     // block starts with as many (a setmaxnreg.inc beyond them would wait forever)
@@ -317,7 +320,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                 };
                 auto products = [&](int i, int b) {
                     const uint64_t vd = v_desc + (uint32_t)((b & 1) * C::KV_STAGE / 16);
-                    const uint32_t o = tmem + 2 * C::TM_S + i * C::TM_O, p = tmem + i * C::TM_S;
+                    const uint32_t o = tmem + 2 * C::TM_S + (i * C::O_BUF + (b & (C::O_BUF - 1))) * C::TM_O, p = tmem + i * C::TM_S;
 #pragma unroll
                     for (int k = 0; k < KVB / 16; k++) {
                         // weights of CH positions: CH / 2 columns of hi, then of lo
@@ -526,7 +529,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
         }
         const float factor = fmaxf(s_factor[128 * i + r], 1e-37f);  // above zero: a masked -infinity times it stays one
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + i * C::TM_S, to = tmem + lanes + 2 * C::TM_S + i * C::TM_O;
+        const uint32_t ts = tmem + lanes + i * C::TM_S, to = tmem + lanes + 2 * C::TM_S + i * C::O_BUF * C::TM_O;
         float m = -INFINITY, l = 0.f;
         float o[HD];
         if constexpr (SPLIT) {
@@ -551,22 +554,23 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                     f(c + 1, rb);
                 }
             };
-            auto add_products = [&]() {  // the last block's, with the factor that its maximum gave
+            auto add_products = [&](int b, float alpha) {  // block b's, with the factor that its maximum gave
+                const uint32_t at = to + (b & (C::O_BUF - 1)) * C::TM_O;
                 auto add = [&](int k, uint32_t x, uint32_t y) {
                     const float2 v = fma2(make_float2(o[k], o[k + 1]), make_float2(alpha, alpha),
                                           make_float2(__uint_as_float(x), __uint_as_float(y)));
                     o[k] = v.x;
                     o[k + 1] = v.y;
                 };
-                tmem_ld_start(to, ra);
+                tmem_ld_start(at, ra);
 #pragma unroll
                 for (int c = 0; c < HD / CH; c += 2) {
                     tmem_ld_wait(ra);
-                    tmem_ld_start(to + CH * (c + 1), rb);
+                    tmem_ld_start(at + CH * (c + 1), rb);
 #pragma unroll
                     for (int k = 0; k < CH; k += 2) add(CH * c + k, ra[k], ra[k + 1]);
                     tmem_ld_wait(rb);
-                    if (c + 2 < HD / CH) tmem_ld_start(to + CH * (c + 2), ra);
+                    if (c + 2 < HD / CH) tmem_ld_start(at + CH * (c + 2), ra);
 #pragma unroll
                     for (int k = 0; k < CH; k += 2) add(CH * (c + 1) + k, rb[k], rb[k + 1]);
                 }
@@ -575,7 +579,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                 ok = kp_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
                 if (!ok) break;
                 tc_fence_after();
-                if (b > 0) add_products();
+                if (C::O_BUF == 1 && b > 0) add_products(b - 1, alpha);
+                const float last = alpha;
                 const int bp = pos0 + b * KVB;
                 float2 sum = make_float2(0.f, 0.f);
                 auto block = [&](auto edge) {
@@ -629,11 +634,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&p_full[i]);
+                if (C::O_BUF == 2 && b > 0) add_products(b - 1, last);
             }
             if (blocks > 0 && ok) {
                 ok = kp_wait(&o_full[i], 0);
                 tc_fence_after();
-                if (ok) add_products();
+                if (ok) add_products(blocks - 1, alpha);
             }
         } else {
             // f16, bf16: O stays in TMEM; m is followed up, and O and l rescaled, only when a maximum exceeds it by 2^8
