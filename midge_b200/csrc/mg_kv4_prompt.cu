@@ -24,10 +24,12 @@
 // and O accumulates in TMEM, whose truncated sums are far finer than either.
 //
 // Measured, one sequence of 4096 new tokens, 64 heads of 64 over 8, f32:
-// 0.34 ms = 405 TFLOP/s, 810 of f16 MMAs; 3 x 1009 tokens behind 5k to 16k,
-// 32 heads of 128 over 4, bf16: 0.51 ms = 1.0 PFLOP/s.  A block of 128 positions
-// takes some 4500 cycles: bound by the chain S -> maximum -> weights -> P V of
-// a tile, of which the other tile hides about half, then by the MUFU; a block
+// 0.33 ms = 415 TFLOP/s, 830 of f16 MMAs; 3 x 1009 tokens behind 5k to 16k,
+// 32 heads of 128 over 4, bf16: 0.475 ms = 1.06 PFLOP/s.  A block of 128 positions
+// takes some 4000 cycles: bound by the chain S -> maximum -> weights -> P V of
+// a tile, of which the other tile hides about half, then by the MUFU; P V of a
+// block's first half starts while the weights of the second are worked out
+// (340 and 507 us without); a block
 // of rows adds some 10 us of its own at start and end.  Blocks of 64 positions
 // measured 6% slower on the first and 24% on the second.
 #include <type_traits>
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     extern __shared__ uint8_t raw_smem[];
     uint8_t *base = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
     uint8_t *sq = base, *sk = base + 2 * C::Q_TILE, *sv = sk + 2 * C::KV_STAGE;
-    __shared__ uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], o_full[2], q_full;
+    __shared__ uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], q_full;
     __shared__ uint32_t tmem_base;
     __shared__ float s_factor[KP_ROWS];
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
@@ -280,6 +282,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
             mbar_init(&k_empty[i], 1);
             mbar_init(&v_empty[i], 1);
             mbar_init(&s_full[i], 1);
+            mbar_init(&p_half[i], 4);
             mbar_init(&p_full[i], 4);
             mbar_init(&o_full[i], 1);
         }
@@ -318,11 +321,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                     }
                     mma_commit(&s_full[i]);
                 };
-                auto products = [&](int i, int b) {
+                auto products = [&](int i, int b, int half) {  // of the first or last positions of a block
                     const uint64_t vd = v_desc + (uint32_t)((b & 1) * C::KV_STAGE / 16);
                     const uint32_t o = tmem + 2 * C::TM_S + (i * C::O_BUF + (b & (C::O_BUF - 1))) * C::TM_O, p = tmem + i * C::TM_S;
 #pragma unroll
-                    for (int k = 0; k < KVB / 16; k++) {
+                    for (int kk = 0; kk < KVB / 32; kk++) {
+                        const int k = half * (KVB / 32) + kk;
                         // weights of CH positions: CH / 2 columns of hi, then of lo
                         const int at = k * 16 / C::CH * C::CH + k * 16 % C::CH / 2;
                         mma_ts(o, p + at, vd + k * 2048 / 16, id_o, k > 0 || (!SPLIT && b > 0));
@@ -342,10 +346,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
 #pragma unroll
                     for (int i = 0; i < 2; i++) {
                         if (b >= u.nb[i] || !ok) continue;
+                        ok = kp_wait(&p_half[i], b & 1);
+                        if (!ok) continue;
+                        tc_fence_after();
+                        products(i, b, 0);
                         ok = kp_wait(&p_full[i], b & 1);
                         if (!ok) continue;
                         tc_fence_after();
-                        products(i, b);
+                        products(i, b, 1);
                         if (b + 1 < u.nb[i]) {
                             ok = kp_wait(&k_full[(b + 1) & 1], ((b + 1) >> 1) & 1);
                             if (ok) scores(i, b + 1);
@@ -532,6 +540,13 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
         const uint32_t ts = tmem + lanes + i * C::TM_S, to = tmem + lanes + 2 * C::TM_S + i * C::O_BUF * C::TM_O;
         float m = -INFINITY, l = 0.f;
         float o[HD];
+        // the weights stored so far are P's (or its first half's)
+        auto weights_out = [&](uint64_t *bar) {
+            tmem_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar);
+        };
         if constexpr (SPLIT) {
             // f32: O in registers, each block's product added with the factor that its maximum gave
             float alpha = 1.f;
@@ -624,16 +639,14 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                             kp_split(e[k], e[k + 1], w[k / 2], w[CH / 2 + k / 2]);
                         }
                         tmem_st(ts + CH * c, w);
+                        if (c == NC / 2 - 1) weights_out(&p_half[i]);
                     });
                 };
                 // some row does not see some position of the block
                 if (bp + KVB - 1 > first_row_p || (a.window > 0 && bp <= last_row_p - a.window)) block(std::true_type{});
                 else block(std::false_type{});
                 l = fmaf(l, alpha, sum.x + sum.y);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[i]);
+                weights_out(&p_full[i]);
                 if (C::O_BUF == 2 && b > 0) add_products(b - 1, last);
             }
             if (blocks > 0 && ok) {
@@ -698,12 +711,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                         w[k / 2] = kp_h2(e.x, e.y);
                     }
                     tmem_st(ts + 32 * c, w);
+                    if (c == KVB / 64 - 1) weights_out(&p_half[i]);
                 }
                 l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                tmem_wait_st();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&p_full[i]);
+                weights_out(&p_full[i]);
             }
 #pragma unroll
             for (int k = 0; k < HD; k++) o[k] = 0.f;
