@@ -645,10 +645,10 @@ static int attn_check(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv, K
 }
 
 // Rows of a key/value head from which the tcgen05 kernel (two tiles of 128
-// rows a block) is taken.  16 sequences of 4096, us with 48, 64 and 96 rows:
-// few-row kernel 77, 97, 139 (f32, head_dim 64) and 57, 66, 86 (bf16, 128),
-// tcgen05 90, 91, 93 and 57, 58, 59; one sequence of 8192: 17, 20, 24 against
-// 29, 29, 30 and 21, 21, 24 against 31, 31, 32.
+// rows a block) is taken.  16 sequences of 4096, us with 48, 64 and 96 rows, f32
+// at head_dim 64: few-row kernel 76, 95, 139, tcgen05 83, 85, 86; at 128: 74, 96
+// against 94, 96 (48 and 64 rows); bf16: 58, 66 against 68, 70 and, at 128, 57, 67
+// against 54, 54; one sequence of 8192 with 64 rows 18 to 22 against 24 to 46.
 constexpr int KV4_MANY_ROWS = 64;
 static bool is_many(int gq, int max_q) { return (int64_t)gq * max_q > KV4_MANY_ROWS; }
 

@@ -29,8 +29,8 @@
 // takes some 4000 cycles: bound by the chain S -> maximum -> weights -> P V of
 // a tile, of which the other tile hides about half, then by the MUFU; P V of a
 // block's first half starts while the weights of the second are worked out
-// (340 and 507 us without); a block
-// of rows adds some 10 us of its own at start and end.  Blocks of 64 positions
+// (340 and 507 us without; quarters measured the same as halves); a block of
+// rows adds some 10 us of its own at start and end.  Blocks of 64 positions
 // measured 6% slower on the first and 24% on the second.
 #include <type_traits>
 
