@@ -58,6 +58,7 @@ struct LpSmem {
     uint16_t who[LP_THREADS];  // threads whose maximum reaches the bound
     float bound;
     int n, nwho, last;
+    int kept;  // candidates that lp_thin keeps: not n, which other warps may still be reading when it starts
 };
 
 __device__ __forceinline__ float lp_ex2(float x) {
@@ -177,7 +178,8 @@ __device__ __forceinline__ void lp_bound(LpSmem &sm, int top) {
 
 // The candidates thinned the way the row was, where there are more than
 // ranking by counting is good for (short rows, whose entries few threads
-// hold): each thread has n / LP_THREADS of them.
+// hold): each thread has n / LP_THREADS of them.  The block's threads
+// together, with the same n: nothing here writes what n was read from.
 constexpr int LP_MANY = 96;
 __device__ __forceinline__ int lp_thin(LpSmem &sm, int n, int top) {
     if (n <= LP_MANY) return n;
@@ -194,7 +196,7 @@ __device__ __forceinline__ int lp_thin(LpSmem &sm, int n, int top) {
 #pragma unroll
     for (int o = LP_LANES / 2; o > 0; o >>= 1) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, o));
     if (threadIdx.x % LP_LANES == 0) sm.gmax[threadIdx.x / LP_LANES] = g;
-    if (threadIdx.x == 0) sm.n = 0;
+    if (threadIdx.x == 0) sm.kept = 0;
     __syncthreads();
     lp_bound(sm, top);
     __syncthreads();
@@ -202,12 +204,12 @@ __device__ __forceinline__ int lp_thin(LpSmem &sm, int n, int top) {
 #pragma unroll
     for (int k = 0; k < K; k++)
         if (id[k] >= 0 && v[k] >= bound) {
-            const int c = atomicAdd(&sm.n, 1);
+            const int c = atomicAdd(&sm.kept, 1);
             sm.cv[c] = v[k];
             sm.ci[c] = id[k];
         }
     __syncthreads();
-    return sm.n;
+    return sm.kept;
 }
 
 // With fewer than `top` possible tokens in [a, b) (n of them, ranked already)
