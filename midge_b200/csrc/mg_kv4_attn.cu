@@ -31,9 +31,11 @@ namespace mg {
 // f32 queries and weights go as f16 hi and lo halves in two MMAs into the
 // same accumulator (22 bits; a tile's sums start from zero and are added in
 // fp32, since the tensor core truncates its running sum).  f16 and bf16
-// queries are exact in f16 after scaling by a power of two per row; their
-// weights are rounded to f16 (2^-11 of a weight: a quarter of the bf16
-// result's own rounding).
+// queries are scaled to f16 by a power of two per row: exact down to 2^-14 of
+// the row's largest, and within 2^-25 of it below.  Their weights are rounded
+// to f16, 2^-11 of a weight: an eighth of a bf16 result's own rounding, and
+// as much as an f16 result's.  Weights are taken 2^15 times as large
+// (KV4_AHEAD), so that small ones keep these bits too.
 //
 // Work: a unit is a (sequence, key/value head, row group); units of more than
 // `chunk` tiles are cut into equal pieces, chunk coming from the tiles of the
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
                     top.x = fmaxf(top.x, __shfl_xor_sync(0xffffffffu, top.x, x));
                     top.y = fmaxf(top.y, __shfl_xor_sync(0xffffffffu, top.y, x));
                 }
-                top = mul2(top, factor[s]);
+                top = fma2_up(top, factor[s], make_float2(-KV4_AHEAD, -KV4_AHEAD));
                 const float2 mn = make_float2(fmaxf(m[s].x, top.x), fmaxf(m[s].y, top.y));
                 float2 mm = mn;  // -infinity only where a row has seen nothing yet
                 if (EDGE) mm = make_float2(mn.x == -INFINITY ? 0.f : mn.x, mn.y == -INFINITY ? 0.f : mn.y);

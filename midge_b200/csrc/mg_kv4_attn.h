@@ -50,6 +50,18 @@ struct Kv4Seq {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
+// Softmax weights go to the tensor cores in f16, whose grid ends at 2^-24: a
+// weight 2^(x - max) below that would vanish from the products while the sum
+// still counts it, and many such make a tail that matters (32768 positions
+// 17.5 nats below a first one: 8e-4 of the result).  So the reference m of a
+// row's weights 2^(x - m) lies KV4_AHEAD below its largest x: weights of up to
+// 2^15, nothing lost above 2^-40 of the largest.  m, sums and outputs go
+// together, so the joins and sinks need no correction.  m is rounded up:
+// x - m is never above KV4_AHEAD, whatever the size of x (f16 ends at 65504).
+// Where m may lag behind the largest x by KV4_LAG (the many-row kernel for
+// 16-bit types) it starts that much higher, and 2^-32 of the largest is kept.
+constexpr float KV4_AHEAD = 15.f, KV4_LAG = 8.f;
+
 // N consecutive elements as floats; 16 bytes at a time where the row allows
 template <int N, typename T>
 __device__ __forceinline__ void load_row(const T *src, bool wide, float x[N]) {

@@ -20,7 +20,7 @@
 // fp32, since the tensor core truncates its running sum.  f16 and bf16: a
 // query is exact in f16 after scaling by a power of two per row (what falls
 // below f16's range is 2^-24 of the row's largest), weights are rounded to
-// f16 (2^-11, below the result's own rounding in bf16 and like it in f16)
+// f16 (2^-11, an eighth of the result's own rounding in bf16 and like it in f16)
 // and O accumulates in TMEM, whose truncated sums are far finer than either.
 //
 // Measured, one sequence of 4096 new tokens, 64 heads of 64 over 8, f32:
@@ -615,7 +615,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                         for (int k = 0; k < 4; k += 2) t4[k] = max3(t4[k], __uint_as_float(r[12 + k]), __uint_as_float(r[13 + k]));
                         top = max3(top, max3(t4[0], t4[1], t4[2]), t4[3]);
                     });
-                    const float mn = top == -INFINITY ? m : fmaxf(m, top * factor), mm = mn == -INFINITY ? 0.f : mn;
+                    const float mn = top == -INFINITY ? m : fmaxf(m, __fmaf_ru(top, factor, -KV4_AHEAD));
+                    const float mm = mn == -INFINITY ? 0.f : mn;
                     alpha = kp_ex2(m - mm);
                     m = mn;
                     columns(edge, [&](int c, uint32_t (&r)[CH]) {
@@ -655,8 +656,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                 if (ok) add_products(blocks - 1, alpha);
             }
         } else {
-            // f16, bf16: O stays in TMEM; m is followed up, and O and l rescaled, only when a maximum exceeds it by 2^8
-            // (weights up to 256 keep their 11 bits in f16)
+            // f16, bf16: O stays in TMEM; m is followed up, and O and l rescaled, only when the largest x is more than KV4_LAG
+            // above the one that m was taken from (weights of up to 2^15 all the same)
             for (int b = 0; b < blocks; b++) {
                 ok = kp_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
                 if (!ok) break;
@@ -680,8 +681,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
 #pragma unroll
                     for (int k = 0; k < 32; k += 2) t4[c] = max3(t4[c], __uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1]));
                 }
-                const float top = max3(fmaxf(t4[0], t4[1]), t4[2], t4[3]), need = top == -INFINITY ? -INFINITY : top * factor;
-                if (__any_sync(0xffffffffu, need > m + 8.f)) {  // m = -infinity: any number
+                const float top = max3(fmaxf(t4[0], t4[1]), t4[2], t4[3]), need = top == -INFINITY ? -INFINITY : __fmaf_ru(top, factor, KV4_LAG - KV4_AHEAD);
+                if (__any_sync(0xffffffffu, need - m > KV4_LAG)) {  // m = -infinity: any number
                     const float mn = fmaxf(m, need), alpha = mn == -INFINITY ? 1.f : kp_ex2(m - mn);
                     m = mn;
                     l *= alpha;
