@@ -211,13 +211,22 @@ int mg_kv4_read(const mg_kv4 *c, int act, int n_tok, const int32_t *tok_seq, con
  * stream, of whatever sizes it is large enough for.  Calls that overlap in
  * time need a workspace each.  A call launches one or two kernels, allocates
  * nothing and waits for nothing, so it may be captured in a CUDA graph; the
- * first call of a process on a device sets kernel attributes and allocates the
- * library's error word, so it comes before any capture.  Results do not depend
- * on the order in which blocks run: the same call gives the same bits. */
+ * first call of a process on a device sets kernel attributes, so it comes
+ * before any capture.  Results do not depend on the order in which blocks run:
+ * the same call gives the same bits.  The kernels' own waits are bounded; one
+ * that runs out leaves wrong rows and marks the workspace, which
+ * mg_kv4_attn_status tells. */
 int64_t mg_kv4_attn_work(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv);
 int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q, int64_t ldq, const int32_t *q_start,
                 const int32_t *kv_len, int max_q, int64_t max_kv, float scale, int window, const float *sinks,
                 void *out, int64_t ldo, void *work, int64_t work_bytes, void *stream);
+
+/* Waits for the stream, then: MG_OK, or MG_ERR_TIMEOUT where a wait inside a
+ * mg_kv4_attn call with this workspace ran out since it was last zero (none
+ * does on a healthy device); outputs since then are not to be used, and the
+ * workspace (work_bytes of it) is zeroed for the next call.  Not for use
+ * during a capture. */
+int mg_kv4_attn_status(void *work, int64_t work_bytes, void *stream);
 
 /* Per logits row (row i at logits + i * ldl, V entries): the natural-log
  * probabilities of its n_ids given tokens ids[i * n_ids ..] (an id outside

@@ -112,6 +112,7 @@ def _load():
         "mg_kv4_attn_work": (i64, [C.POINTER(MgKv4), i32, i32, i64]),
         "mg_kv4_attn": (i32, [C.POINTER(MgKv4), i32, i32, vp, i64, vp, vp, i32, i64, f32, i32, vp, vp, i64, vp, i64,
                               vp]),
+        "mg_kv4_attn_status": (i32, [vp, i64, vp]),
         "mg_logprobs_work": (i64, [i64, i32, i32]),
         "mg_logprobs": (i32, [i32, vp, i64, i64, i32, vp, i32, i32, vp, vp, vp, vp, vp, i64, vp]),
         "mg_wait_selftest": (i32, [i32, C.POINTER(i32)]),

@@ -9,7 +9,6 @@
 // and 0 where it sees nothing.  The head h reads key/value head h / gq.
 #include <type_traits>
 
-#include "mg_kernels.h"
 #include "mg_kv4_attn.h"
 #include "mg_tc.cuh"
 
@@ -654,9 +653,10 @@ static int attn_check(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv, K
 constexpr int KV4_MANY_ROWS = 64;
 static bool is_many(int gq, int max_q) { return (int64_t)gq * max_q > KV4_MANY_ROWS; }
 
-// The workspace: partial results of the most pieces of any call, so that the
-// counters behind them lie in the same place for every call, and a counter
-// per (sequence, key/value head, row group).  Pieces of cut units are at most
+// The workspace: partial results of the most pieces of any call, so that what
+// is behind them lies in the same place for every call: the status word (the
+// code of a wait that ran out, 0: none), and a counter per (sequence,
+// key/value head, row group).  Pieces of cut units are at most
 // twice FewCut::pieces (a unit of n > 1 pieces has more than n / 2 chunks);
 // the many-row kernel has its own bound and no counters.
 static int64_t attn_part_bytes() {
@@ -665,8 +665,9 @@ static int64_t attn_part_bytes() {
     const int64_t few = 2 * KD_WAVES * (d64 > d128 ? d64 : d128) * 4, many = kv4_many_part_floats(num_sms()) * 4;
     return few > many ? few : many;
 }
+constexpr int64_t KV4_STATUS_BYTES = 16;
 static int64_t attn_work(const Kv4 &c, int groups) {
-    return attn_part_bytes() + (int64_t)c.n_seqs * c.n_kv * groups * 4;
+    return attn_part_bytes() + KV4_STATUS_BYTES + (int64_t)c.n_seqs * c.n_kv * groups * 4;
 }
 
 }  // namespace mg
@@ -705,12 +706,11 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
     a.window = window;
     a.sinks = sinks;
     a.parts = static_cast<float *>(work);
-    a.count = reinterpret_cast<unsigned *>(static_cast<uint8_t *>(work) + attn_part_bytes());
+    a.err = reinterpret_cast<int *>(static_cast<uint8_t *>(work) + attn_part_bytes());
+    a.count = reinterpret_cast<unsigned *>(a.err + KV4_STATUS_BYTES / 4);
     const int64_t size = act == MG_ACT_F32 ? 4 : 2;
     a.q_wide = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(ldq * size)) & 15) == 0;
     a.out_wide = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * size)) & 15) == 0;
-    a.err = stream_error_word();
-    MG_REQUIRE(a.err, MG_ERR_OOM, "kv4_attn: no error word");
     cudaStream_t st = (cudaStream_t)stream;
     if (is_many(a.gq, max_q)) return kv4_attn_many(a, c->head_dim, act, max_kv, st);
     const int mode = few_mode(act, a.gq, max_q);
@@ -718,4 +718,19 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
     if (act == MG_ACT_F32) return attn_few<float>(a, c->head_dim, mode, f, st);
     if (act == MG_ACT_F16) return attn_few<__half>(a, c->head_dim, mode, f, st);
     return attn_few<__nv_bfloat16>(a, c->head_dim, mode, f, st);
+}
+
+extern "C" int mg_kv4_attn_status(void *work, int64_t work_bytes, void *stream) {
+    const int64_t at = attn_part_bytes();
+    MG_REQUIRE(work && work_bytes >= at + KV4_STATUS_BYTES && (reinterpret_cast<uintptr_t>(work) & 15) == 0, MG_ERR_ARG,
+               "kv4_attn_status: %lld bytes, not a workspace of kv4_attn", (long long)(work ? work_bytes : 0));
+    cudaStream_t st = (cudaStream_t)stream;
+    int code = 0;
+    MG_CUDA(cudaMemcpyAsync(&code, static_cast<uint8_t *>(work) + at, sizeof(int), cudaMemcpyDeviceToHost, st));
+    MG_CUDA(cudaStreamSynchronize(st));
+    if (!code) return MG_OK;
+    MG_CUDA(cudaMemsetAsync(work, 0, (size_t)work_bytes, st));
+    MG_CUDA(cudaStreamSynchronize(st));
+    set_error("kv4_attn: a bounded wait timed out (code %d)", code);
+    return MG_ERR_TIMEOUT;
 }

@@ -24,7 +24,7 @@ struct Kv4AttnArgs {
     unsigned *count;
     int row_groups;   // the most row groups of a sequence
     int pieces, min_chunk;  // pieces wanted of the whole call, and the least tiles of one
-    int *err;
+    int *err;  // the workspace's status word
 };
 
 // rows (query, head) that a kernel holds at a time, and the floats of one of its partial results:

@@ -34,7 +34,6 @@
 // measured 6% slower on the first and 24% on the second.
 #include <type_traits>
 
-#include "mg_kernels.h"
 #include "mg_kv4_attn.h"
 #include "mg_tc.cuh"
 

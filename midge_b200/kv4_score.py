@@ -165,6 +165,7 @@ class Kv4Model:
                                      h.data_ptr(), x.data_ptr(), self.stream))
         out = torch.empty(n, f["vocab"], device="cuda")
         self._gemv("lm_head", self._norm(x, "final_norm"), out)
+        abi.check(lib.mg_kv4_attn_status(self.work.data_ptr(), self.work.numel(), self.stream))
         return out
 
 
