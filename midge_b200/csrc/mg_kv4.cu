@@ -182,18 +182,32 @@ __device__ __forceinline__ void append_queries(const AppendArgs &a, int share) {
         load_f32<V, WIDE>(a.q_norm + d + HALF, w1);
 #pragma unroll
         for (int k = 0; k < AP_HEADS; k++) {
-            float2 s2 = make_float2(0.f, 0.f);
+            auto mean_square = [&] {
+                float2 s2 = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < V; i++) {
-                const float2 v = make_float2(x0[k][i], x1[k][i]);
-                s2 = fma2(v, v, s2);
+                for (int i = 0; i < V; i++) {
+                    const float2 v = make_float2(x0[k][i], x1[k][i]);
+                    s2 = fma2(v, v, s2);
+                }
+                float ss = s2.x + s2.y;
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
+                return ss * (1.0f / HD);
+            };
+            float mean = mean_square() + a.eps;
+            // squares beyond fp32 (or, with an eps of nothing, below it): the head times a power of two, which drops out again
+            const bool far = !(mean < 0x1p127f) || mean < 0x1p-100f;
+            if (__any_sync(~0u, far)) {
+                const float f = !far ? 1.f : mean < 1.f ? 0x1p100f : 0x1p-80f;
+#pragma unroll
+                for (int i = 0; i < V; i++) {
+                    x0[k][i] *= f;
+                    x1[k][i] *= f;
+                }
+                mean = mean_square() + a.eps * f * f;
             }
-            float ss = s2.x + s2.y;
-#pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(~0u, ss, o);
-            const float mean = ss * (1.0f / HD) + a.eps;
             float inv = rsqrtf(mean);  // and a Newton step
-            inv = mean > 0.f && inv < INFINITY ? inv * fmaf(-0.5f * mean * inv, inv, 1.5f) : inv;
+            inv = mean > 0.f && mean < INFINITY ? inv * fmaf(-0.5f * mean * inv, inv, 1.5f) : inv;
             const float2 i2 = make_float2(inv, inv);
 #pragma unroll
             for (int i = 0; i < V; i += 2) {
