@@ -70,11 +70,12 @@ __device__ __forceinline__ bool better(float v, int32_t i, float w, int32_t j) {
 // NaN counts as -infinity
 __device__ __forceinline__ float clean(float x) { return fmaxf(x, -INFINITY); }
 
-// sum and weighted sum against a maximum m, moved to the maximum M >= m
+// Sum and weighted sum against a maximum m, moved to the maximum M >= m.  Where nothing is left of them (87 or more
+// apart, m = -infinity among these) they are 0: s times such a d may pass fp32.
 __device__ __forceinline__ void lp_move(float &s, float &w, float m, float M) {
-    const float d = fmaxf(m - M, -1e30f), f = lp_ex2(d * LP_LOG2E);  // m = -infinity: s = w = 0, and f is 0
-    w = f * (w + s * d);
-    s *= f;
+    const float d = fmaxf(m - M, -1e30f), f = lp_ex2(d * LP_LOG2E);
+    w = f > 0.f ? f * (w + s * d) : 0.f;
+    s = f > 0.f ? f * s : 0.f;
 }
 
 // A thread's sums are against a reference r that follows its maximum m only when that is LP_AHEAD above it (e^40 times the
