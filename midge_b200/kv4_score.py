@@ -188,6 +188,9 @@ def logprobs(logits, ids, top: int):
 def score(model: Kv4Model, ids, seq: int = 0, top: int = 5, step: int = STEP):
     """What the model says of ids[1:], each from the tokens before it: arrays
     of log probability, entropy, alternatives and theirs, one row a token."""
+    # step looks at all but the last, which mg_logprobs would take for "no token": probability 1
+    if len(ids) < 2 or any(not 0 <= t < model.f["vocab"] for t in ids):
+        raise ValueError("two tokens of the vocabulary at least")
     parts = []
     for a in range(0, len(ids) - 1, step):
         t = list(ids[a:min(a + step, len(ids) - 1)])
