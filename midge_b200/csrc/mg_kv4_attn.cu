@@ -655,8 +655,8 @@ static bool is_many(int gq, int max_q) { return (int64_t)gq * max_q > KV4_MANY_R
 
 // The workspace: partial results of the most pieces of any call, so that what
 // is behind them lies in the same place for every call: the status word (the
-// code of a wait that ran out, 0: none), and a counter per (sequence,
-// key/value head, row group).  Pieces of cut units are at most
+// code of a wait that ran out, 0: none), the many-row kernel's marks of taken
+// places, and a counter per (sequence, key/value head, row group).  Pieces of cut units are at most
 // twice FewCut::pieces (a unit of n > 1 pieces has more than n / 2 chunks);
 // the many-row kernel has its own bound and no counters.
 static int64_t attn_part_bytes() {
@@ -666,9 +666,7 @@ static int64_t attn_part_bytes() {
     return few > many ? few : many;
 }
 constexpr int64_t KV4_STATUS_BYTES = 16;
-static int64_t attn_work(const Kv4 &c, int groups) {
-    return attn_part_bytes() + KV4_STATUS_BYTES + (int64_t)c.n_seqs * c.n_kv * groups * 4;
-}
+static int64_t attn_work(int64_t units) { return attn_part_bytes() + KV4_STATUS_BYTES + (num_sms() + units) * 4; }
 
 }  // namespace mg
 
@@ -677,7 +675,7 @@ using namespace mg;
 extern "C" int64_t mg_kv4_attn_work(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv) {
     Kv4 k;
     TRY(attn_check(c, n_heads, max_q, max_kv, &k));
-    return attn_work(k, ceil_div((int64_t)max_q * (n_heads / c->n_kv_heads), 8));
+    return attn_work((int64_t)k.n_seqs * k.n_kv * ceil_div((int64_t)max_q * (n_heads / c->n_kv_heads), 8));
 }
 
 extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q, int64_t ldq, const int32_t *q_start,
@@ -691,7 +689,7 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
                "kv4_attn: bad arguments");
     a.gq = n_heads / c->n_kv_heads;
     a.row_groups = ceil_div((int64_t)max_q * a.gq, 8);
-    const int64_t need = attn_work(a.c, a.row_groups);
+    const int64_t need = attn_work((int64_t)a.c.n_seqs * a.c.n_kv * a.row_groups);
     MG_REQUIRE(work && work_bytes >= need && (reinterpret_cast<uintptr_t>(work) & 15) == 0, MG_ERR_ARG,
                "kv4_attn: %lld bytes of workspace (16-byte aligned), need %lld", (long long)(work ? work_bytes : 0), (long long)need);
     a.n_heads = n_heads;
@@ -707,7 +705,8 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
     a.sinks = sinks;
     a.parts = static_cast<float *>(work);
     a.err = reinterpret_cast<int *>(static_cast<uint8_t *>(work) + attn_part_bytes());
-    a.count = reinterpret_cast<unsigned *>(a.err + KV4_STATUS_BYTES / 4);
+    a.taken = reinterpret_cast<unsigned *>(a.err + KV4_STATUS_BYTES / 4);
+    a.count = a.taken + num_sms();
     const int64_t size = act == MG_ACT_F32 ? 4 : 2;
     a.q_wide = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(ldq * size)) & 15) == 0;
     a.out_wide = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * size)) & 15) == 0;
@@ -721,12 +720,11 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
 }
 
 extern "C" int mg_kv4_attn_status(void *work, int64_t work_bytes, void *stream) {
-    const int64_t at = attn_part_bytes();
-    MG_REQUIRE(work && work_bytes >= at + KV4_STATUS_BYTES && (reinterpret_cast<uintptr_t>(work) & 15) == 0, MG_ERR_ARG,
+    MG_REQUIRE(work && work_bytes >= attn_work(1) && (reinterpret_cast<uintptr_t>(work) & 15) == 0, MG_ERR_ARG,
                "kv4_attn_status: %lld bytes, not a workspace of kv4_attn", (long long)(work ? work_bytes : 0));
     cudaStream_t st = (cudaStream_t)stream;
     int code = 0;
-    MG_CUDA(cudaMemcpyAsync(&code, static_cast<uint8_t *>(work) + at, sizeof(int), cudaMemcpyDeviceToHost, st));
+    MG_CUDA(cudaMemcpyAsync(&code, static_cast<uint8_t *>(work) + attn_part_bytes(), sizeof(int), cudaMemcpyDeviceToHost, st));
     MG_CUDA(cudaStreamSynchronize(st));
     if (!code) return MG_OK;
     MG_CUDA(cudaMemsetAsync(work, 0, (size_t)work_bytes, st));

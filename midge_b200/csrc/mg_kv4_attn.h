@@ -25,6 +25,7 @@ struct Kv4AttnArgs {
     int row_groups;   // the most row groups of a sequence
     int pieces, min_chunk;  // pieces wanted of the whole call, and the least tiles of one
     int *err;  // the workspace's status word
+    unsigned *taken;  // of the many-row kernel's places for long sums, one per SM: 1 while a block has it
 };
 
 // rows (query, head) that a kernel holds at a time, and the floats of one of its partial results:

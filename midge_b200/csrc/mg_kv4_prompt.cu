@@ -21,7 +21,8 @@
 // query is exact in f16 after scaling by a power of two per row (what falls
 // below f16's range is 2^-24 of the row's largest), weights are rounded to
 // f16 (2^-11, an eighth of the result's own rounding in bf16 and like it in f16)
-// and O accumulates in TMEM, whose truncated sums are far finer than either.
+// and O accumulates in TMEM for KP_RUN blocks at a time: truncated sums, off by
+// 9e-5 at worst.
 //
 // Measured, one sequence of 4096 new tokens, 64 heads of 64 over 8, f32:
 // 0.33 ms = 415 TFLOP/s, 830 of f16 MMAs; 3 x 1009 tokens behind 5k to 16k,
@@ -42,7 +43,10 @@ namespace mg {
 constexpr int KP_ROWS = 256;        // rows of a block
 constexpr int KP_THREADS = 512;
 constexpr int KP_DEQ = 7;           // warps 8-14
-constexpr int KP_ERR = 42;
+constexpr int KP_ERR = 42, KP_PLACE_ERR = 43;
+// Blocks that 16-bit types sum in TMEM at a stretch, a power of two: 9e-5 lost at worst, a fifth of f16's rounding.  Three
+// chunks behind 5k to 16k: 536 us as with sums of any length, with half as many 545.
+constexpr int KP_RUN = 128;
 
 template <int HD, bool SPLIT>
 struct KpCfg {
@@ -256,6 +260,20 @@ struct KpUnit {
     }
 };
 
+// A place for a block's long sums among those for the pieces' results, which a call that cuts nothing leaves free: one
+// per SM, and an SM holds one block, so there is always a free one but for the time that a block takes to leave.
+constexpr uint32_t KP_PLACE_POLLS = 1u << 20;
+__device__ __forceinline__ int kp_take_place(const Kv4AttnArgs &a, int slots) {
+    int s = blockIdx.x % slots;
+    for (uint32_t i = 0; i < KP_PLACE_POLLS; i++, s = s + 1 < slots ? s + 1 : 0)
+        if (atomicExch(&a.taken[s], 1u) == 0u) {
+            __threadfence();
+            return s;
+        }
+    atomicExch(a.err, KP_PLACE_ERR);
+    return s;
+}
+
 template <int HD, bool SPLIT, typename T>
 __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, int row_tiles, int cuts, int slots, int part_rows) {
     using C = KpCfg<HD, SPLIT>;
@@ -266,6 +284,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     __shared__ uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_half[2], p_full[2], o_full[2], q_full;
     __shared__ uint32_t tmem_base;
     __shared__ float s_factor[KP_ROWS];
+    __shared__ int s_place;
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
     __shared__ KpPlan plan;
@@ -273,6 +292,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     {
         KpUnit<KVB> u;
         if (!u.load(a, plan, blockIdx.x, row_tiles, cuts)) return;  // the whole block
+        if (tid == 0) s_place = cuts > 1 ? (int)blockIdx.x : !SPLIT && u.nblk > KP_RUN ? kp_take_place(a, slots) : -1;
     }
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -328,7 +348,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
                         const int k = half * (KVB / 32) + kk;
                         // weights of CH positions: CH / 2 columns of hi, then of lo
                         const int at = k * 16 / C::CH * C::CH + k * 16 % C::CH / 2;
-                        mma_ts(o, p + at, vd + k * 2048 / 16, id_o, k > 0 || (!SPLIT && b > 0));
+                        mma_ts(o, p + at, vd + k * 2048 / 16, id_o, k > 0 || (!SPLIT && (b & (KP_RUN - 1)) > 0));
                         if (SPLIT) mma_ts(o, p + at + C::CH / 2, vd + k * 2048 / 16, id_o, 1u);
                     }
                 };
@@ -656,65 +676,116 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
             }
         } else {
             // f16, bf16: O stays in TMEM; m is followed up, and O and l rescaled, only when the largest x is more than KV4_LAG
-            // above the one that m was taken from (weights of up to 2^15 all the same)
-            for (int b = 0; b < blocks; b++) {
-                ok = kp_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
-                if (!ok) break;
-                tc_fence_after();
-                uint32_t r[KVB / 32][32];
+            // above the one that m was taken from (weights of up to 2^15 all the same).
+            // The tensor core truncates its running sum, some 2^-22.5 of it with each MMA: values of one sign lose 5.4e-9 of
+            // theirs a position (measured: 7e-4 of 131072).  So after KP_RUN blocks O goes to the row's place in memory,
+            // against `rest_m`, and the next products start from zero.
+            float rest_m = -INFINITY;
+            // (a warp's rows share the part that its results go to in the end, four columns of each side by side)
+            const int near = min(32, part_rows - (128 * i + (r & ~31)));
+            auto place = [&](int c) {
+                return a.parts + (size_t)s_place * part_rows * (HD + 2) + 2 * part_rows + (128 * i + (r & ~31)) * HD +
+                       c * near + lane * 4;
+            };
+            auto add_rest = [&](float *x, int c, float f) {  // columns c .. c + 31 of what rests, times f
 #pragma unroll
-                for (int c = 0; c < KVB / 32; c++) tmem_ld_start(ts + 32 * c, r[c]);
-#pragma unroll
-                for (int c = 0; c < KVB / 32; c++) tmem_ld_wait(r[c]);
-                const int bp = pos0 + b * KVB;
-                // some row does not see some position of the block
-                if (bp + KVB - 1 > first_row_p || (a.window > 0 && bp <= last_row_p - a.window)) {
-                    const int up = hi - bp, down = lo - bp;
-#pragma unroll
-                    for (int k = 0; k < KVB; k++) r[k / 32][k % 32] = k <= up && k >= down ? r[k / 32][k % 32] : 0xff800000u;
+                for (int k = 0; k < 32; k += 4) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(place(c + k)));
+                    x[k] = fmaf(v.x, f, x[k]);
+                    x[k + 1] = fmaf(v.y, f, x[k + 1]);
+                    x[k + 2] = fmaf(v.z, f, x[k + 2]);
+                    x[k + 3] = fmaf(v.w, f, x[k + 3]);
                 }
-                float t4[4];
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    t4[c] = -INFINITY;
-#pragma unroll
-                    for (int k = 0; k < 32; k += 2) t4[c] = max3(t4[c], __uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1]));
-                }
-                const float top = max3(fmaxf(t4[0], t4[1]), t4[2], t4[3]), need = top == -INFINITY ? -INFINITY : __fmaf_ru(top, factor, KV4_LAG - KV4_AHEAD);
-                if (__any_sync(0xffffffffu, need - m > KV4_LAG)) {  // m = -infinity: any number
-                    const float mn = fmaxf(m, need), alpha = mn == -INFINITY ? 1.f : kp_ex2(m - mn);
-                    m = mn;
-                    l *= alpha;
-                    if (b > 0) {
+            };
+            auto rest_factor = [&] { return m == -INFINITY ? 0.f : kp_ex2(rest_m - m); };
+            auto put_to_rest = [&](bool first) {  // O, whose products are complete
+                const float f = rest_factor();
 #pragma unroll 1
-                        for (int c = 0; c < HD; c += 16) {
-                            uint32_t v[16];
-                            tmem_ld_start(to + c, v);
-                            tmem_ld_wait(v);
+                for (int c = 0; c < HD; c += 32) {
+                    uint32_t v[32];
+                    tmem_ld_start(to + c, v);
+                    tmem_ld_wait(v);
+                    float x[32];
 #pragma unroll
-                            for (int k = 0; k < 16; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
-                            tmem_st(to + c, v);
+                    for (int k = 0; k < 32; k++) x[k] = __uint_as_float(v[k]);
+                    if (live) {
+                        if (!first) add_rest(x, c, f);
+#pragma unroll
+                        for (int k = 0; k < 32; k += 4)
+                            __stcg(reinterpret_cast<float4 *>(place(c + k)), make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]));
+                    }
+                    __syncwarp();
+                }
+                rest_m = m;
+            };
+            for (int b = 0, run = 0; b < blocks && ok; run = b) {
+                if (run > 0) {
+                    ok = kp_wait(&s_full[i], b & 1);
+                    if (!ok) break;
+                    tc_fence_after();
+                    put_to_rest(run == KP_RUN);
+                }
+                const int end = min(blocks, run + KP_RUN);
+                for (; b < end; b++) {
+                    ok = kp_wait(&s_full[i], b & 1);  // implies that the block before's products are complete
+                    if (!ok) break;
+                    tc_fence_after();
+                    uint32_t r[KVB / 32][32];
+#pragma unroll
+                    for (int c = 0; c < KVB / 32; c++) tmem_ld_start(ts + 32 * c, r[c]);
+#pragma unroll
+                    for (int c = 0; c < KVB / 32; c++) tmem_ld_wait(r[c]);
+                    const int bp = pos0 + b * KVB;
+                    // some row does not see some position of the block
+                    if (bp + KVB - 1 > first_row_p || (a.window > 0 && bp <= last_row_p - a.window)) {
+                        const int up = hi - bp, down = lo - bp;
+#pragma unroll
+                        for (int k = 0; k < KVB; k++) r[k / 32][k % 32] = k <= up && k >= down ? r[k / 32][k % 32] : 0xff800000u;
+                    }
+                    float t4[4];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        t4[c] = -INFINITY;
+#pragma unroll
+                        for (int k = 0; k < 32; k += 2) t4[c] = max3(t4[c], __uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1]));
+                    }
+                    const float top = max3(fmaxf(t4[0], t4[1]), t4[2], t4[3]);
+                    const float need = top == -INFINITY ? -INFINITY : __fmaf_ru(top, factor, KV4_LAG - KV4_AHEAD);
+                    if (__any_sync(0xffffffffu, need - m > KV4_LAG)) {  // m = -infinity: any number
+                        const float mn = fmaxf(m, need), alpha = mn == -INFINITY ? 1.f : kp_ex2(m - mn);
+                        m = mn;
+                        l *= alpha;
+                        if (b > run) {
+#pragma unroll 1
+                            for (int c = 0; c < HD; c += 16) {
+                                uint32_t v[16];
+                                tmem_ld_start(to + c, v);
+                                tmem_ld_wait(v);
+#pragma unroll
+                                for (int k = 0; k < 16; k++) v[k] = __float_as_uint(__uint_as_float(v[k]) * alpha);
+                                tmem_st(to + c, v);
+                            }
                         }
                     }
-                }
-                const float mm = m == -INFINITY ? 0.f : m;
-                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                    const float mm = m == -INFINITY ? 0.f : m;
+                    float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
-                for (int c = 0; c < KVB / 32; c++) {
-                    uint32_t w[16];
+                    for (int c = 0; c < KVB / 32; c++) {
+                        uint32_t w[16];
 #pragma unroll
-                    for (int k = 0; k < 32; k += 2) {
-                        const float2 x = fma2(make_float2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])),
-                                              make_float2(factor, factor), make_float2(-mm, -mm));
-                        const float2 e = make_float2(kp_ex2(x.x), kp_ex2(x.y));
-                        sum[k / 2 % 2] = add2(sum[k / 2 % 2], e);
-                        w[k / 2] = kp_h2(e.x, e.y);
+                        for (int k = 0; k < 32; k += 2) {
+                            const float2 x = fma2(make_float2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])),
+                                                  make_float2(factor, factor), make_float2(-mm, -mm));
+                            const float2 e = make_float2(kp_ex2(x.x), kp_ex2(x.y));
+                            sum[k / 2 % 2] = add2(sum[k / 2 % 2], e);
+                            w[k / 2] = kp_h2(e.x, e.y);
+                        }
+                        tmem_st(ts + 32 * c, w);
+                        if (c == KVB / 64 - 1) weights_out(&p_half[i]);
                     }
-                    tmem_st(ts + 32 * c, w);
-                    if (c == KVB / 64 - 1) weights_out(&p_half[i]);
+                    l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    weights_out(&p_full[i]);
                 }
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
-                weights_out(&p_full[i]);
             }
 #pragma unroll
             for (int k = 0; k < HD; k++) o[k] = 0.f;
@@ -730,6 +801,12 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
 #pragma unroll
                         for (int k = 0; k < 32; k++) o[c + k] = __uint_as_float(v[k]);
                     }
+                    if (blocks > KP_RUN && live) {
+                        const float f = rest_factor();
+#pragma unroll
+                        for (int c = 0; c < HD; c += 32) add_rest(o + c, c, f);
+                    }
+                    __syncwarp();  // all have read: a piece's results may go there
                 }
             }
         }
@@ -763,6 +840,10 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     if (warp == 15) {
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
+    }
+    if (cuts == 1 && tid == 0 && s_place >= 0) {
+        __threadfence();
+        atomicExch(&a.taken[s_place], 0u);
     }
 }
 
