@@ -51,7 +51,7 @@ namespace mg {
 // from codes to fragments, which is why codes lie in fragment order and a
 // warp shares no tile with another.
 constexpr int KD_NST = 4;    // ring stages of a warp
-constexpr int KD_ERR = 41;
+constexpr int KD_ERR = 41, KD_PLACE_ERR = 44;
 constexpr int KD_WARPS_LONG = 4, KD_WARPS_SHORT = 2;  // warps of a block
 // Tiles worth a piece of their own where blocks would be idle, and where they
 // would not: a piece costs about as much as 16 tiles (five queries each of 16
@@ -59,6 +59,13 @@ constexpr int KD_WARPS_LONG = 4, KD_WARPS_SHORT = 2;  // warps of a block
 // up to 32768: 135 either way).
 constexpr int KD_MIN_CHUNK = 16, KD_LONG_CHUNK = 64;
 constexpr int KD_MAX_CUT = 128;                       // pieces of a unit
+// Tiles that a warp sums at a stretch in 16-bit types.  The tensor core truncates its running sum: values of one sign
+// lose 1.7e-7 of theirs a tile of the warp's, 9e-5 here (measured without stretches: 6.9e-4 of 4096 tiles, 524288
+// positions of each of 320 sequences).  A longer piece is done in several goes, whose sums rest in the block's place.
+// The loop over goes costs 1 to 3% (16 x 5 queries 63.6 -> 65.1 us), so calls whose table holds no longer piece go
+// without it.
+constexpr int KD_RUN = 512;
+__host__ __device__ constexpr int kd_rest_floats(int hd) { return 16 * hd / 4 * 6; }  // a place: four outputs, maximum and sum a thread
 __host__ __device__ constexpr int kd_warps_sm(int hd) { return hd == 64 ? 16 : 12; }  // 128 and 168 registers a thread
 
 enum { KD_SPLIT = 0, KD_ROWS8 = 1, KD_ROWS16 = 2 };
@@ -114,7 +121,7 @@ __device__ __forceinline__ uint32_t live_bytes(uint32_t w, int p, int first, int
     return w;
 }
 
-template <int HD, int MODE, typename T, int KD_WARPS>
+template <int HD, int MODE, typename T, int KD_WARPS, bool GOES>
 __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_kv4_attn_few(Kv4AttnArgs a) {
     constexpr int KD_THREADS = KD_WARPS * 32;
     constexpr int ROWS = kd_rows(MODE), SETS = ROWS / 8, TB = kv4_tile_bytes(HD), KS = HD / 16, G = HD / 32;
@@ -125,8 +132,9 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
     __shared__ long long s_sum[KD_WARPS];
     __shared__ int2 s_scan[KD_WARPS];
     __shared__ Kv4Seq s_q;
-    __shared__ int s_seq, s_off, s_slot, s_last;
+    __shared__ int s_seq, s_off, s_slot, s_last, s_place;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    if (GOES && tid == 0) s_place = -1;
     uint8_t *ring = smem + (size_t)warp * KD_NST * TB;
     if (lane == 0) {
         for (int i = 0; i < KD_NST; i++) mbar_init(&bars[warp][i], 1);
@@ -182,7 +190,8 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
 
     uint32_t phase = 0;  // bit i: parity of ring stage i's next completion
     bool ok = true;
-    for (int piece = blockIdx.x; piece < total; piece += gridDim.x) {
+    [[maybe_unused]] int done = 0;  // tiles of the piece that earlier goes did
+    for (int piece = blockIdx.x; piece < total;) {
         if (piece >= excl.x && piece < excl.x + mine.x) {
             int at = excl.x, slot = excl.y;
             for (int s = s0;; s++) {
@@ -206,8 +215,12 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
         const int groups = q.groups(a.gq, ROWS), ncut = cuts(q);
         const int hr = s_off / ncut, cut = s_off - hr * ncut;
         const int kh = hr / groups, rg = hr - kh * groups;
-        const int ta = (int)((long long)q.tiles * cut / ncut), nt = (int)((long long)q.tiles * (cut + 1) / ncut) - ta;
-        const int tile_a = q.tile0 + ta;
+        const int ta = (int)((long long)q.tiles * cut / ncut);
+        const int piece_tiles = (int)((long long)q.tiles * (cut + 1) / ncut) - ta;
+        constexpr int GO = KD_WARPS * KD_RUN;  // tiles of a go
+        if (GOES && tid == 0 && piece_tiles > GO && s_place < 0) s_place = kv4_take_place(a, KD_PLACE_ERR);
+        const int nt = GOES ? min(GO, piece_tiles - done) : piece_tiles, tile_a = q.tile0 + ta + (GOES ? done : 0);
+        const bool last_go = !GOES || nt == piece_tiles - done;
         const int wt = nt > warp ? (nt - warp + KD_WARPS - 1) / KD_WARPS : 0;  // this warp's tiles of it
 
         // ---- bulk copies: lane i keeps the address of the warp's tile base + i
@@ -506,6 +519,22 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
                 L += all[w * WS + ROWS + r] * e;
                 acc.x += v.x * e; acc.y += v.y * e; acc.z += v.z * e; acc.w += v.w * e;
             }
+            if (GOES && piece_tiles > GO) {  // with what rests of the goes before, or to rest
+                float *at = a.rest + (size_t)s_place * kd_rest_floats(HD) + i, *ml = at - i + 16 * HD + i / 2;
+                if (done > 0) {
+                    const float4 v = __ldcg(reinterpret_cast<const float4 *>(at));
+                    const float2 s = __ldcg(reinterpret_cast<const float2 *>(ml));
+                    const float M2 = fmaxf(M, s.x), m2 = M2 == -INFINITY ? 0.f : M2, e = ex2(M - m2), f = ex2(s.x - m2);
+                    M = M2;
+                    L = L * e + s.y * f;
+                    acc.x = acc.x * e + v.x * f; acc.y = acc.y * e + v.y * f; acc.z = acc.z * e + v.z * f; acc.w = acc.w * e + v.w * f;
+                }
+                if (!last_go) {
+                    __stcg(reinterpret_cast<float4 *>(at), acc);
+                    __stcg(reinterpret_cast<float2 *>(ml), make_float2(M, L));
+                    continue;
+                }
+            }
             if (!whole) {
                 *reinterpret_cast<float4 *>(part + 2 * ROWS + i) = acc;
                 if (dd == 0) {
@@ -524,7 +553,7 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
                         make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
             }
         }
-        if (!whole) {
+        if (!whole && last_go) {
             __threadfence();
             __syncthreads();
             if (tid == 0) {
@@ -569,7 +598,10 @@ __global__ void __launch_bounds__(KD_WARPS * 32, kd_warps_sm(HD) / KD_WARPS) k_k
         }
         fence_proxy_async_smem();  // the rings held the results: copies may fill them again
         __syncthreads();
+        done = last_go ? 0 : done + nt;
+        if (last_go) piece += gridDim.x;
     }
+    if (GOES && tid == 0 && s_place >= 0) kv4_leave_place(a, s_place);
     if (!ok) {  // a wait ran out: the copies still on their way, then out
         for (int i = 0; i < KD_NST; i++) {
             mbar_wait(&bars[warp][i], ((phase >> i) & 1) ^ 1);
@@ -605,14 +637,22 @@ static FewCut few_cut(const Kv4 &c, int gq, int rows, int max_q, int64_t max_kv,
     return f;
 }
 
-template <int HD, int MODE, typename T, int WARPS>
+template <int HD, int MODE, typename T, int WARPS, bool GOES>
 static int launch_few(Kv4AttnArgs &a, const FewCut &f, cudaStream_t st) {
     a.pieces = f.pieces;
     a.min_chunk = f.min_chunk;
-    TRY(ensure_smem(k_kv4_attn_few<HD, MODE, T, WARPS>, kd_smem<HD>(WARPS)));
-    k_kv4_attn_few<HD, MODE, T, WARPS><<<f.blocks, WARPS * 32, kd_smem<HD>(WARPS), st>>>(a);
+    a.places = few_most(HD, WARPS);
+    TRY(ensure_smem(k_kv4_attn_few<HD, MODE, T, WARPS, GOES>, kd_smem<HD>(WARPS)));
+    k_kv4_attn_few<HD, MODE, T, WARPS, GOES><<<f.blocks, WARPS * 32, kd_smem<HD>(WARPS), st>>>(a);
     MG_CHECK_LAUNCH();
     return MG_OK;
+}
+template <int HD, int MODE, typename T, int WARPS>
+static int launch_few(Kv4AttnArgs &a, const FewCut &f, cudaStream_t st) {
+    if constexpr (MODE != KD_SPLIT) {  // f32 adds each tile's sums in fp32
+        if (a.c.cap > (int64_t)WARPS * KD_RUN * KV4_TILE) return launch_few<HD, MODE, T, WARPS, true>(a, f, st);
+    }
+    return launch_few<HD, MODE, T, WARPS, false>(a, f, st);
 }
 template <int HD, int MODE, typename T>
 static int launch_few(Kv4AttnArgs &a, const FewCut &f, cudaStream_t st) {
@@ -655,10 +695,11 @@ static bool is_many(int gq, int max_q) { return (int64_t)gq * max_q > KV4_MANY_R
 
 // The workspace: partial results of the most pieces of any call, so that what
 // is behind them lies in the same place for every call: the status word (the
-// code of a wait that ran out, 0: none), the many-row kernel's marks of taken
-// places, and a counter per (sequence, key/value head, row group).  Pieces of cut units are at most
-// twice FewCut::pieces (a unit of n > 1 pieces has more than n / 2 chunks);
-// the many-row kernel has its own bound and no counters.
+// code of a wait that ran out, 0: none), the marks of taken places and the
+// few-row kernel's places, and a counter per (sequence, key/value head, row
+// group).  Pieces of cut units are at most twice FewCut::pieces (a unit of
+// n > 1 pieces has more than n / 2 chunks); the many-row kernel has its own
+// bound and no counters.
 static int64_t attn_part_bytes() {
     const int64_t d64 = (int64_t)few_most(64, KD_WARPS_LONG) * kv4_part_floats(16, 64);
     const int64_t d128 = (int64_t)few_most(128, KD_WARPS_LONG) * kv4_part_floats(16, 128);
@@ -666,7 +707,15 @@ static int64_t attn_part_bytes() {
     return few > many ? few : many;
 }
 constexpr int64_t KV4_STATUS_BYTES = 16;
-static int64_t attn_work(int64_t units) { return attn_part_bytes() + KV4_STATUS_BYTES + (num_sms() + units) * 4; }
+static int attn_places() { return few_most(64, KD_WARPS_SHORT); }  // the most blocks of any kernel here at a time
+static int64_t attn_rest_bytes() {
+    const int64_t d64 = (int64_t)few_most(64, KD_WARPS_SHORT) * kd_rest_floats(64);
+    const int64_t d128 = (int64_t)few_most(128, KD_WARPS_SHORT) * kd_rest_floats(128);
+    return (d64 > d128 ? d64 : d128) * 4;
+}
+static int64_t attn_work(int64_t units) {
+    return attn_part_bytes() + KV4_STATUS_BYTES + attn_places() * 4 + attn_rest_bytes() + units * 4;
+}
 
 }  // namespace mg
 
@@ -706,11 +755,13 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
     a.parts = static_cast<float *>(work);
     a.err = reinterpret_cast<int *>(static_cast<uint8_t *>(work) + attn_part_bytes());
     a.taken = reinterpret_cast<unsigned *>(a.err + KV4_STATUS_BYTES / 4);
-    a.count = a.taken + num_sms();
+    a.rest = reinterpret_cast<float *>(a.taken + attn_places());
+    a.count = reinterpret_cast<unsigned *>(reinterpret_cast<uint8_t *>(a.rest) + attn_rest_bytes());
     const int64_t size = act == MG_ACT_F32 ? 4 : 2;
     a.q_wide = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(ldq * size)) & 15) == 0;
     a.out_wide = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * size)) & 15) == 0;
     cudaStream_t st = (cudaStream_t)stream;
+    a.places = num_sms();  // the many-row kernel's
     if (is_many(a.gq, max_q)) return kv4_attn_many(a, c->head_dim, act, max_kv, st);
     const int mode = few_mode(act, a.gq, max_q);
     const FewCut f = few_cut(a.c, a.gq, kd_rows(mode), max_q, max_kv, window, c->head_dim);

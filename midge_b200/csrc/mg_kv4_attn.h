@@ -25,8 +25,31 @@ struct Kv4AttnArgs {
     int row_groups;   // the most row groups of a sequence
     int pieces, min_chunk;  // pieces wanted of the whole call, and the least tiles of one
     int *err;  // the workspace's status word
-    unsigned *taken;  // of the many-row kernel's places for long sums, one per SM: 1 while a block has it
+    // places where blocks keep the sums of what they have done of a long piece: `places` of them, as many as blocks fit
+    // the GPU, each with a word that is 1 while a block has it; the few-row kernel's places lie in `rest`, the many-row
+    // kernel's among the pieces' results
+    unsigned *taken;
+    int places;
+    float *rest;
 };
+
+// A free place for this block (one thread of it).  There is one but for the time that a block takes to leave; a place
+// is held to the block's end, by kv4_leave_place after a barrier of its threads.
+constexpr uint32_t KV4_PLACE_POLLS = 1u << 20;
+__device__ __forceinline__ int kv4_take_place(const Kv4AttnArgs &a, int err) {
+    int s = blockIdx.x % a.places;
+    for (uint32_t i = 0; i < KV4_PLACE_POLLS; i++, s = s + 1 < a.places ? s + 1 : 0)
+        if (atomicExch(&a.taken[s], 1u) == 0u) {
+            __threadfence();
+            return s;
+        }
+    atomicExch(a.err, err);
+    return s;
+}
+__device__ __forceinline__ void kv4_leave_place(const Kv4AttnArgs &a, int s) {
+    __threadfence();
+    atomicExch(&a.taken[s], 0u);
+}
 
 // rows (query, head) that a kernel holds at a time, and the floats of one of its partial results:
 // the rows' maxima and sums, then their outputs

@@ -260,20 +260,6 @@ struct KpUnit {
     }
 };
 
-// A place for a block's long sums among those for the pieces' results, which a call that cuts nothing leaves free: one
-// per SM, and an SM holds one block, so there is always a free one but for the time that a block takes to leave.
-constexpr uint32_t KP_PLACE_POLLS = 1u << 20;
-__device__ __forceinline__ int kp_take_place(const Kv4AttnArgs &a, int slots) {
-    int s = blockIdx.x % slots;
-    for (uint32_t i = 0; i < KP_PLACE_POLLS; i++, s = s + 1 < slots ? s + 1 : 0)
-        if (atomicExch(&a.taken[s], 1u) == 0u) {
-            __threadfence();
-            return s;
-        }
-    atomicExch(a.err, KP_PLACE_ERR);
-    return s;
-}
-
 template <int HD, bool SPLIT, typename T>
 __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, int row_tiles, int cuts, int slots, int part_rows) {
     using C = KpCfg<HD, SPLIT>;
@@ -292,7 +278,8 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
     {
         KpUnit<KVB> u;
         if (!u.load(a, plan, blockIdx.x, row_tiles, cuts)) return;  // the whole block
-        if (tid == 0) s_place = cuts > 1 ? (int)blockIdx.x : !SPLIT && u.nblk > KP_RUN ? kp_take_place(a, slots) : -1;
+        // a piece's long sums rest where its result goes; a call that cuts nothing leaves those places free, one per SM
+        if (tid == 0) s_place = cuts > 1 ? (int)blockIdx.x : !SPLIT && u.nblk > KP_RUN ? kv4_take_place(a, KP_PLACE_ERR) : -1;
     }
     if (tid == 0) {
         for (int i = 0; i < 2; i++) {
@@ -841,10 +828,7 @@ __global__ void __launch_bounds__(KP_THREADS, 1) k_kv4_attn_many(Kv4AttnArgs a, 
         tc_fence_after();
         tmem_dealloc(tmem_base, 512);
     }
-    if (cuts == 1 && tid == 0 && s_place >= 0) {
-        __threadfence();
-        atomicExch(&a.taken[s_place], 0u);
-    }
+    if (cuts == 1 && tid == 0 && s_place >= 0) kv4_leave_place(a, s_place);
 }
 
 template <int N> __device__ __forceinline__ void load_f(const float *src, float v[N]) {
