@@ -146,8 +146,8 @@ int mg_sample_topp(const float *logits, int64_t ldl, int64_t V, int n_rows, floa
 /* ---- 4-bit paged key/value cache and token scoring (no counterpart in the
  * reference, whose cache is f16 and contiguous, engine/midge.c:267-273, and
  * which reports logits only).  Rows of activations (queries, keys, values,
- * outputs, logits) are f32, f16 or bf16; sums, softmax statistics and norms
- * are 32 bits or more whatever the type. */
+ * outputs, logits) are f32, f16 or bf16, each row aligned to its type; sums,
+ * softmax statistics and norms are 32 bits or more whatever the type. */
 enum { MG_ACT_F32 = 0, MG_ACT_F16 = 1, MG_ACT_BF16 = 2 };
 
 /* A layer's cache: a pool of pages shared by n_seqs sequences.  Position p of

@@ -424,6 +424,8 @@ extern "C" int mg_kv4_append(const mg_kv4 *c, int act, int n_tok, int n_heads, c
                MG_ERR_ARG, "kv4_append: bad arguments");
     MG_REQUIRE(n_heads == 0 || (q && q_out && ldq >= q_dim && ldqo >= q_dim), MG_ERR_ARG,
                "kv4_append: %d query heads need q and q_out rows", n_heads);
+    MG_REQUIRE(act_aligned(q, act) && act_aligned(k, act) && act_aligned(v, act) && act_aligned(q_out, act), MG_ERR_ARG,
+               "kv4_append: rows not aligned to their type");
     MG_REQUIRE(!rope_cos == !rope_sin && (!rope_cos || rope_rows >= 1), MG_ERR_ARG,
                "kv4_append: rope_cos and rope_sin go together");
     MG_REQUIRE(!(eps < 0.f), MG_ERR_ARG, "kv4_append: eps %g", (double)eps);
@@ -446,7 +448,7 @@ extern "C" int mg_kv4_append(const mg_kv4 *c, int act, int n_tok, int n_heads, c
     a.seq = tok_seq;
     a.pos = tok_pos;
     a.q_out = q_out;
-    const int size = act == MG_ACT_F32 ? 4 : 2;
+    const int size = act_size(act);
     a.wide = wide_rows(size, {k, v}, {ldk, ldv}) && (n_heads == 0 || wide_rows(size, {q, q_out}, {ldq, ldqo})) &&
              wide_rows(4, {q_norm, k_norm, rope_cos, rope_sin}, {});
     cudaStream_t st = (cudaStream_t)stream;
@@ -463,6 +465,7 @@ extern "C" int mg_kv4_read(const mg_kv4 *c, int act, int n_tok, const int32_t *t
     MG_REQUIRE(act >= MG_ACT_F32 && act <= MG_ACT_BF16, MG_ERR_ARG, "kv4_read: activation type %d", act);
     MG_REQUIRE(n_tok >= 0 && tok_pos && (k || v) && (!k || ldk >= kv_dim) && (!v || ldv >= kv_dim), MG_ERR_ARG,
                "kv4_read: bad arguments");
+    MG_REQUIRE(act_aligned(k, act) && act_aligned(v, act), MG_ERR_ARG, "kv4_read: rows not aligned to their type");
     if (n_tok == 0) return MG_OK;
     a.n_tok = n_tok;
     a.seq = tok_seq;
@@ -471,7 +474,7 @@ extern "C" int mg_kv4_read(const mg_kv4 *c, int act, int n_tok, const int32_t *t
     a.v = v;
     a.ldk = ldk;
     a.ldv = ldv;
-    const int size = act == MG_ACT_F32 ? 4 : 2;
+    const int size = act_size(act);
     a.wide = (!k || wide_rows(size, {k}, {ldk})) && (!v || wide_rows(size, {v}, {ldv}));
     cudaStream_t st = (cudaStream_t)stream;
     if (act == MG_ACT_F32) return read_t<float>(a, c->head_dim, st);

@@ -134,6 +134,10 @@ template <> __device__ __forceinline__ float from_f32<float>(float x) { return x
 template <> __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// bytes of an activation type's element, and whether a row of them can start at p (a kernel's load elsewhere would fault)
+inline int act_size(int act) { return act == MG_ACT_F32 ? 4 : 2; }
+inline bool act_aligned(const void *p, int act) { return reinterpret_cast<uintptr_t>(p) % act_size(act) == 0; }
+
 // The cache as the kernels take it.  Table entries are clamped to the pool,
 // so that a stale entry reads another page but never outside the pool.
 struct Kv4 {

@@ -736,6 +736,7 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
     MG_REQUIRE(act >= MG_ACT_F32 && act <= MG_ACT_BF16, MG_ERR_ARG, "kv4_attn: activation type %d", act);
     MG_REQUIRE(q && out && q_start && kv_len && ldq >= dim && ldo >= dim && window >= 0, MG_ERR_ARG,
                "kv4_attn: bad arguments");
+    MG_REQUIRE(act_aligned(q, act) && act_aligned(out, act), MG_ERR_ARG, "kv4_attn: rows not aligned to their type");
     a.gq = n_heads / c->n_kv_heads;
     a.row_groups = ceil_div((int64_t)max_q * a.gq, 8);
     const int64_t need = attn_work((int64_t)a.c.n_seqs * a.c.n_kv * a.row_groups);
@@ -757,7 +758,7 @@ extern "C" int mg_kv4_attn(const mg_kv4 *c, int act, int n_heads, const void *q,
     a.taken = reinterpret_cast<unsigned *>(a.err + KV4_STATUS_BYTES / 4);
     a.rest = reinterpret_cast<float *>(a.taken + attn_places());
     a.count = reinterpret_cast<unsigned *>(reinterpret_cast<uint8_t *>(a.rest) + attn_rest_bytes());
-    const int64_t size = act == MG_ACT_F32 ? 4 : 2;
+    const int64_t size = act_size(act);
     a.q_wide = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)(ldq * size)) & 15) == 0;
     a.out_wide = ((reinterpret_cast<uintptr_t>(out) | (uintptr_t)(ldo * size)) & 15) == 0;
     cudaStream_t st = (cudaStream_t)stream;

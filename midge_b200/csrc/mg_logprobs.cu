@@ -533,6 +533,7 @@ extern "C" int mg_logprobs(int act, const void *logits, int64_t ldl, int64_t V, 
     MG_REQUIRE(logits && ldl >= V && entropy && n_ids >= 0 && (n_ids == 0 || (ids && lp)) &&
                    (n_alt == 0 || (alt_ids && alt_lp)),
                MG_ERR_ARG, "logprobs: bad arguments");
+    MG_REQUIRE(act_aligned(logits, act), MG_ERR_ARG, "logprobs: rows not aligned to their type");
     const int64_t need = mg_logprobs_work(V, n_rows, n_alt);
     MG_REQUIRE(work && work_bytes >= need && (reinterpret_cast<uintptr_t>(work) & 15) == 0, MG_ERR_ARG,
                "logprobs: %lld bytes of workspace (16-byte aligned), need %lld", (long long)(work ? work_bytes : 0),
