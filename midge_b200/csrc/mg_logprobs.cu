@@ -27,7 +27,10 @@ namespace mg {
 
 constexpr int LP_THREADS = 512;
 constexpr int LP_GROUPS = 64, LP_LANES = LP_THREADS / LP_GROUPS;  // groups of 8 lanes, one maximum each
-constexpr int LP_CAND = 1024;                                     // candidates that fit shared memory
+// Candidates that fit shared memory: whole rows of up to 2048 entries, since 16-bit rows below that have their vectors in
+// fewer groups than there may be alternatives, so that every entry is one (2048 rows of 1500, 32 alternatives: 294 us with
+// room for 1024)
+constexpr int LP_CAND = 2048;
 constexpr int LP_UNROLL = 4;                                      // 16-byte loads of a thread in flight
 constexpr int LP_MAX_PARTS = 1024, LP_MAX_ROWS = 512;             // of a call that cuts rows
 constexpr float LP_LOG2E = 1.4426950408889634f;
