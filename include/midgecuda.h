@@ -147,7 +147,11 @@ int mg_sample_topp(const float *logits, int64_t ldl, int64_t V, int n_rows, floa
  * reference, whose cache is f16 and contiguous, engine/midge.c:267-273, and
  * which reports logits only).  Rows of activations (queries, keys, values,
  * outputs, logits) are f32, f16 or bf16, each row aligned to its type; sums,
- * softmax statistics and norms are 32 bits or more whatever the type. */
+ * softmax statistics and norms are 32 bits or more whatever the type.  What
+ * is not: attention's weights, which go to the tensor cores with 22 bits for
+ * f32 and with 11 for f16 and bf16 (2^-12 of each, unbiased), and for the
+ * latter two its running sums, which are fp32 but truncated (up to 9e-5 of
+ * like-signed values). */
 enum { MG_ACT_F32 = 0, MG_ACT_F16 = 1, MG_ACT_BF16 = 2 };
 
 /* A layer's cache: a pool of pages shared by n_seqs sequences.  Position p of
@@ -205,7 +209,10 @@ int mg_kv4_read(const mg_kv4 *c, int act, int n_tok, const int32_t *tok_seq, con
  * logits that join each softmax without a value.  A query that sees nothing
  * gets zeros.  max_q >= every number of queries (rows beyond it are not
  * written) and max_kv, about the longest kv_len, choose the kernel and its
- * split; any kv_len up to ld_table * page_size is right.
+ * split; any kv_len up to ld_table * page_size is right.  They hold for the
+ * whole call: single tokens behind long caches are faster in a call of their
+ * own than together with prompt chunks (a cache with their rows of the page
+ * table, or copies of these).
  * work: mg_kv4_attn_work() bytes of device memory (never 0), 16-byte aligned,
  * zero before its first use; a call leaves it ready for the next on the same
  * stream, of whatever sizes it is large enough for.  Calls that overlap in

@@ -54,10 +54,10 @@ struct AppendArgs {
 // they take longer), so that no block has both.
 // Bound: HBM (rows in, queries out; the codes are a tenth), which takes many
 // threads in flight.  Measured with the read back: 4096 tokens, 64 + 2 x 8 heads
-// of 64, f32: 36.5 us (165 MB, 4.5 TB/s); 8191 tokens, 32 + 2 x 4 heads of 128
-// with norms, bf16: 50 us (181 MB, 3.6 TB/s: the norms and the keys' 64-bit
-// arithmetic share the issue slots); 8 tokens: 5.2 us, two launches of two
-// dependent loads.  A query head a thread: 39 and 59 us, three or four heads 36
+// of 64, f32: 37 us (165 MB, 4.5 TB/s; the read 4.4); 8191 tokens, 32 + 2 x 4
+// heads of 128 with norms, bf16: 51 us (181 MB, 3.5 TB/s: the norms and the
+// keys' 64-bit arithmetic share the issue slots; the read 6.1); 8 tokens: 5.3
+// us, two launches of two dependent loads.  A query head a thread: 39 and 59 us, three or four heads 36
 // and 63 or more (16-bit rows spill).
 constexpr int AP_THREADS = 128, AP_HEADS = 2;
 
@@ -320,7 +320,9 @@ struct ReadArgs {
     bool wide;
 };
 
-// thread = eight dimensions of a token's key and value head
+// thread = eight dimensions of a token's key and value head.  Bound: HBM and
+// latency (8191 tokens of 4 heads of 128 to bf16: 6.1 us, 21 MB; 8 tokens 2.5
+// us, a launch)
 template <int HD, typename T, bool WIDE>
 __global__ void __launch_bounds__(256) k_kv4_read(ReadArgs a) {
     constexpr int L = HD / 8;

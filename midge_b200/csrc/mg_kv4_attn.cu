@@ -46,10 +46,12 @@ namespace mg {
 // Measured: 8 sequences of 4096, 64 heads of 64 over 8, f32: 13.8 us (17.8 MB,
 // 1.3 TB/s: launch, the pieces' table, first tiles and the join are 10 of
 // them); 64 sequences of up to 32768, 32 heads of 128 over 4, bf16: 135 us
-// (571 MB, 4.2 TB/s); 128 with a window of 128: 11 us.  Bound there by
-// issue: some 560 instructions a tile of 34 HD bytes, half of them the way
-// from codes to fragments, which is why codes lie in fragment order and a
-// warp shares no tile with another.
+// (571 MB, 4.2 TB/s); 128 with a window of 128: 11 us (one round of blocks of
+// two warps, each mostly prologue).  Bound on the long ones by latency: a
+// tile of 34 HD bytes takes some 560 instructions, half of them the way from
+// codes to fragments (which is why codes lie in fragment order and a warp
+// shares no tile with another), in chains that the 12 to 16 warps which the
+// registers allow fill to 54% of the issue slots, the tensor pipe to 25%.
 constexpr int KD_NST = 4;    // ring stages of a warp
 constexpr int KD_ERR = 41, KD_PLACE_ERR = 44;
 constexpr int KD_WARPS_LONG = 4, KD_WARPS_SHORT = 2;  // warps of a block
@@ -690,6 +692,12 @@ static int attn_check(const mg_kv4 *c, int n_heads, int max_q, int64_t max_kv, K
 // at head_dim 64: few-row kernel 76, 95, 139, tcgen05 83, 85, 86; at 128: 74, 96
 // against 94, 96 (48 and 64 rows); bf16: 58, 66 against 68, 70 and, at 128, 57, 67
 // against 54, 54; one sequence of 8192 with 64 rows 18 to 22 against 24 to 46.
+// The kernel is chosen for the whole call, by its largest number of queries.
+// A call that mixes single tokens behind long caches with a prompt chunk
+// sends all of them to the 256-row blocks, uncut: 63 tokens behind up to
+// 32768 positions and a chunk of 512 behind 20k take 1288 us in one call, 178
+// and 341 in two (f32, 64 heads of 64 over 8; bf16, 32 of 128 over 4: 717,
+// 137 and 175).
 constexpr int KV4_MANY_ROWS = 64;
 static bool is_many(int gq, int max_q) { return (int64_t)gq * max_q > KV4_MANY_ROWS; }
 

@@ -25,8 +25,8 @@
 // 9e-5 at worst.
 //
 // Measured, one sequence of 4096 new tokens, 64 heads of 64 over 8, f32:
-// 0.33 ms = 415 TFLOP/s, 830 of f16 MMAs; 3 x 1009 tokens behind 5k to 16k,
-// 32 heads of 128 over 4, bf16: 0.475 ms = 1.06 PFLOP/s.  A block of 128 positions
+// 0.33 ms = 414 TFLOP/s, 830 of f16 MMAs; 3 x 1009 tokens behind 5k to 16k,
+// 32 heads of 128 over 4, bf16: 0.49 ms = 1.03 PFLOP/s.  A block of 128 positions
 // takes some 4000 cycles: bound by the chain S -> maximum -> weights -> P V of
 // a tile, of which the other tile hides about half, then by the MUFU; P V of a
 // block's first half starts while the weights of the second are worked out
